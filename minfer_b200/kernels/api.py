@@ -7,8 +7,9 @@ library that cannot be built or loaded.
 from __future__ import annotations
 
 import ctypes
+import math
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
-from typing import Optional
+from typing import Dict, NamedTuple, Optional
 
 import torch
 
@@ -391,7 +392,28 @@ def _sig_moe(lib: ctypes.CDLL) -> None:
                                    c_int, c_void_p]
 
 
-_SIGNATURES = {"retention": _sig_retention, "outer_scan": _sig_outer_scan, "delta_rule": _sig_delta_rule, "attention_talk": _sig_attention_talk, "moe": _sig_moe,
+def _sig_cache_q8(lib: ctypes.CDLL) -> None:
+    lib.mf_rope_kvstore_q8.argtypes = ([c_void_p, c_int] + [c_void_p] * 13 + [c_int] * 11 +
+                                       [c_void_p, c_void_p])
+    lib.mf_read_pages_q8.argtypes = ([c_void_p] * 5 + [c_int] * 3 + [c_void_p] * 3 + [c_int] * 6 +
+                                     [c_void_p, c_void_p])
+
+
+def _sig_attention_q8(lib: ctypes.CDLL) -> None:
+    lib.mf_attention_q8_plan.argtypes = [c_int] * 7 + [c_void_p, c_void_p]
+    lib.mf_attention_q8.argtypes = ([c_void_p] * 8 + [c_int] * 3 + [c_void_p, c_void_p] + [c_int] * 9 +
+                                    [c_float, c_int, c_int, c_void_p, c_void_p])
+
+
+def _sig_drafts(lib: ctypes.CDLL) -> None:
+    lib.mf_draft_pieces.argtypes = [c_int]
+    lib.mf_verify_drafts.argtypes = [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_void_p,
+                                     c_void_p, ctypes.c_double, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                                     c_void_p]
+
+
+_SIGNATURES = {"cache_q8": _sig_cache_q8, "attention_q8": _sig_attention_q8, "drafts": _sig_drafts,
+               "retention": _sig_retention, "outer_scan": _sig_outer_scan, "delta_rule": _sig_delta_rule, "attention_talk": _sig_attention_talk, "moe": _sig_moe,
                "attention_prefill_tc": _sig_attention_prefill_tc, "recurrent": _sig_recurrent,
                "mixer_prep": _sig_mixer_prep,
                "attention_sink": _sig_attention_sink, "attention_latent": _sig_attention_latent,
@@ -1059,6 +1081,215 @@ def attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         int(chunk), int(n_chunks), float(scale), dtype_code(q.dtype), 1 if force_generic else 0,
         int(k_cache.shape[0]), _i32(status, "status"), 1 if old_keys_final else 0,
         _stream()), "attention_paged", 2 if n_chunks > 1 else 1)
+
+
+# ---------------------------------------------------------------------------------------
+# 8-bit cache (csrc/cache_q8.cu, csrc/attention_q8.cu)
+# ---------------------------------------------------------------------------------------
+Q8_FORMATS = {torch.float8_e4m3fn: 0, torch.int8: 1}
+
+
+class Q8Pages(NamedTuple):
+    """One cache entry's pages in 8 bits.  A vector (one position of one key/value head) is ``head_dim``
+    codes and a float32 scale, x = code * scale: with a = max(max |x|, 2^-100), scale = a / L and
+    code = round(x * (L / a)), L = 448 (e4m3) or 127 (int8).  A code is off by half a step at most: 2^-4 of the
+    value in e4m3, scale / 2 in int8.  A vector that holds an infinity or a NaN is kept as codes of zero with
+    a scale of NaN and reads back as NaN; nothing that does not see it is touched by it.  Scales are not
+    negative."""
+
+    k: torch.Tensor             # float8_e4m3fn or int8 [pages, n_kv, 64, head_dim]
+    v: torch.Tensor
+    k_scale: torch.Tensor       # float32 [pages, n_kv, 64]
+    v_scale: torch.Tensor
+
+
+def q8_pages(n_pages: int, n_kv: int, head_dim: int, dtype: torch.dtype,
+             device: torch.device | str = "cuda") -> Q8Pages:
+    """Pages of zeros in ``dtype`` (torch.float8_e4m3fn or torch.int8)."""
+    if dtype not in Q8_FORMATS:
+        raise KernelError(f"8-bit pages are float8_e4m3fn or int8, not {dtype}")
+    shape = (n_pages, n_kv, PAGE, head_dim)
+
+    def codes() -> torch.Tensor:
+        return torch.zeros(shape, dtype=torch.int8, device=device).view(dtype)
+
+    def scales() -> torch.Tensor:
+        return torch.zeros(shape[:3], dtype=torch.float32, device=device)
+    return Q8Pages(codes(), codes(), scales(), scales())
+
+
+def _q8(pages: Q8Pages, n_kv: int, head_dim: int, what: str) -> int:
+    """The pages' format, after a look at their types and shapes."""
+    fmt = Q8_FORMATS.get(pages.k.dtype)
+    if fmt is None or pages.v.dtype != pages.k.dtype:
+        raise KernelError(f"{what}: 8-bit pages are float8_e4m3fn or int8, K and V alike")
+    shape = pages.k.shape
+    if len(shape) != 4 or shape[0] < 1 or shape[1:] != (n_kv, PAGE, head_dim) or pages.v.shape != shape:
+        raise KernelError(f"{what}: pages must be [pages, {n_kv}, {PAGE}, {head_dim}]")
+    if pages.k_scale.shape != shape[:3] or pages.v_scale.shape != shape[:3]:
+        raise KernelError(f"{what}: a scale belongs to every vector of the pages")
+    if pages.k_scale.dtype != torch.float32 or pages.v_scale.dtype != torch.float32:
+        raise KernelError(f"{what}: scales must be float32")
+    return fmt
+
+
+def _here(t: torch.Tensor, what: str) -> None:
+    """Launches go to the current device's stream: the tensors must live there."""
+    if not t.is_cuda:
+        raise KernelError(f"{what}: tensors must live on a CUDA device (there is no CPU path)")
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: the tensors live on {t.device}, which is not the current device")
+
+
+def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    _here(first, what)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise KernelError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def _table(page_table: torch.Tensor, table_stride: int, rows: int, what: str) -> None:
+    if table_stride < 1 or page_table.numel() < rows * table_stride:
+        raise KernelError(f"{what}: the page table is smaller than {rows} rows of {table_stride} pages")
+
+
+def rope_kvstore_q8(qkv: torch.Tensor, positions: torch.Tensor, token_row: torch.Tensor,
+                    seq_end: torch.Tensor, inv_freq: Optional[torch.Tensor], q_out: torch.Tensor,
+                    k_out: Optional[torch.Tensor], v_out: Optional[torch.Tensor], pages: Q8Pages,
+                    page_table: torch.Tensor, table_stride: int, ring: int, n_heads: int, n_kv: int,
+                    head_dim: int, rotary_dim: int, style: int, status: torch.Tensor,
+                    n_partials: int = 0, bias: Optional[torch.Tensor] = None) -> None:
+    """``rope_kvstore`` into 8-bit pages: q (and, where given, the step's own k and v) in the
+    activations' type, keys and values quantised from float32 and written at their positions.  What it
+    reads before the kernel in front of it has ended is what ``rope_kvstore`` reads then.  A position without
+    a page is not written and sets status bit 2."""
+    what = "rope_kvstore_q8"
+    if n_partials > 0:
+        if qkv.dim() != 3 or qkv.shape[0] != n_partials:
+            raise KernelError(f"{what}: partial sums must be [splits, tokens, width]")
+        n, width = qkv.shape[1], qkv.shape[2]
+    else:
+        if qkv.dim() != 2:
+            raise KernelError(f"{what}: qkv must be [tokens, width]")
+        n, width = qkv.shape
+    if width != (n_heads + 2 * n_kv) * head_dim:
+        raise KernelError(f"{what}: qkv has the wrong width")
+    if bias is not None and bias.numel() != width:
+        raise KernelError(f"{what}: bias has the wrong length")
+    fmt = _q8(pages, n_kv, head_dim, what)
+    dt = q_out.dtype
+    if q_out.numel() != n * n_heads * head_dim:
+        raise KernelError(f"{what}: q has the wrong size")
+    for t in (k_out, v_out):
+        if t is not None and (t.dtype != dt or t.numel() != n * n_kv * head_dim):
+            raise KernelError(f"{what}: the step's keys and values have another type or size than q")
+    if positions.numel() != n or token_row.numel() != n:
+        raise KernelError(f"{what}: a position and a row belong to every token")
+    if inv_freq is not None and inv_freq.numel() != rotary_dim // 2:
+        raise KernelError(f"{what}: {inv_freq.numel()} frequencies for {rotary_dim} rotated dimensions")
+    if ring < 0 or ring % PAGE != 0:
+        raise KernelError(f"{what}: a ring is whole pages, not {ring} positions")
+    _table(page_table, table_stride, seq_end.numel(), what)
+    _same_device(what, qkv, q_out, k_out, v_out, *pages, positions, token_row, seq_end, page_table, inv_freq, status,
+                 bias)
+    _check(_lib("cache_q8").mf_rope_kvstore_q8(
+        _f32(qkv, "qkv"), int(n_partials), _f32(bias, "bias"), _i32(positions, "positions"),
+        _i32(token_row, "token_row"), _i32(seq_end, "seq_end"), _f64(inv_freq, "inv_freq"), _ptr(q_out, "q_out"),
+        _ptr(k_out, "k_out"), _ptr(v_out, "v_out"), _ptr(pages.k, "keys"), _ptr(pages.v, "values"),
+        _ptr(pages.k_scale, "key scales"), _ptr(pages.v_scale, "value scales"), _i32(page_table, "page_table"),
+        int(table_stride), int(ring), pages.k.shape[0], n, n_heads, n_kv, head_dim, int(rotary_dim), int(style),
+        dtype_code(dt), fmt, _i32(status, "status"), _stream()), what)
+
+
+def read_pages_q8(pages: Q8Pages, page_table: torch.Tensor, table_stride: int, ring: int, seq_end: torch.Tensor,
+                  k_out: torch.Tensor, v_out: torch.Tensor, status: torch.Tensor, fill: bool = True) -> None:
+    """The pages of ``page_table`` read back: ``k_out``, ``v_out`` [rows * table_stride, n_kv, 64, head_dim] in
+    bfloat16 or float32, in the table's order.  Row b holds ``seq_end[b]`` positions; places that hold none
+    are zeros (``fill`` False: pages of which a row holds no position are left as they are).  A page that a
+    row needs and has not reads as zeros and sets status bit 2."""
+    what = "read_pages_q8"
+    if pages.k.dim() != 4:
+        raise KernelError(f"{what}: pages must be [pages, heads, {PAGE}, head size]")
+    n_kv, head_dim = pages.k.shape[1], pages.k.shape[3]
+    fmt = _q8(pages, n_kv, head_dim, what)
+    rows = seq_end.numel()
+    if ring < 0 or ring % PAGE != 0:
+        raise KernelError(f"{what}: a ring is whole pages, not {ring} positions")
+    _table(page_table, table_stride, rows, what)
+    want = rows * table_stride * n_kv * PAGE * head_dim
+    if k_out.dtype != v_out.dtype or k_out.numel() != want or v_out.numel() != want:
+        raise KernelError(f"{what}: the outputs must be [rows * table_stride, {n_kv}, {PAGE}, {head_dim}] of one type")
+    _same_device(what, *pages, page_table, seq_end, k_out, v_out, status)
+    _check(_lib("cache_q8").mf_read_pages_q8(
+        _ptr(pages.k, "keys"), _ptr(pages.v, "values"), _ptr(pages.k_scale, "key scales"),
+        _ptr(pages.v_scale, "value scales"), _i32(page_table, "page_table"), int(table_stride), int(ring),
+        pages.k.shape[0], _i32(seq_end, "seq_end"), _ptr(k_out, "k_out"), _ptr(v_out, "v_out"), rows, n_kv, head_dim,
+        dtype_code(k_out.dtype), fmt, 1 if fill else 0, _i32(status, "status"), _stream()), what)
+
+
+_Q8_PLANS: Dict[tuple, tuple] = {}
+
+
+def attention_q8_plan(n_rows: int, max_row_tokens: int, span: int, n_heads: int, n_kv: int, head_dim: int,
+                      dtype: torch.dtype) -> tuple[int, int]:
+    """(keys of a split, splits) of attention over 8-bit pages; ``span``: the most positions that the queries
+    of a row see."""
+    key = (torch.cuda.current_device(), n_rows, max_row_tokens, span, n_heads, n_kv, head_dim, dtype)
+    got = _Q8_PLANS.get(key)
+    if got is None:
+        chunk, splits = c_int(0), c_int(0)
+        _check(_lib("attention_q8").mf_attention_q8_plan(n_rows, max_row_tokens, span, n_heads, n_kv, head_dim,
+                                                         dtype_code(dtype), ctypes.addressof(chunk),
+                                                         ctypes.addressof(splits)), "attention_q8_plan", 0)
+        got = (chunk.value, splits.value)
+        if len(_Q8_PLANS) > 4096:
+            _Q8_PLANS.clear()
+        _Q8_PLANS[key] = got
+    return got
+
+
+def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor, seq_end: torch.Tensor,
+                       page_table: torch.Tensor, table_stride: int, ring: int, out: torch.Tensor,
+                       max_row_tokens: int, max_end: int, n_heads: int, n_kv: int, head_dim: int, window: int,
+                       scale: float, status: torch.Tensor) -> None:
+    """Attention of a step's tokens over 8-bit pages: row ``b`` brings tokens ``cu_seqlens[b] ..
+    cu_seqlens[b+1]-1`` of ``q`` [tokens, n_heads, head_dim] at positions ``seq_end[b] - count .. seq_end[b] - 1``,
+    and the pages hold every position up to there, the step's own included.  A token sees the positions up
+    to its own (the last ``window`` of them where that is not 0) and reads zeros if there is none.
+    ``max_row_tokens``: the most tokens a row brings; ``max_end``: a bound of ``seq_end`` (it sizes the splits).
+    A page that a token would see and its row has not counts as not seen and sets status bit 2."""
+    what = "attention_paged_q8"
+    rows, tokens = seq_end.numel(), q.shape[0]
+    if n_kv < 1 or n_heads < 1 or n_heads % n_kv != 0:
+        raise KernelError(f"{what}: {n_heads} heads do not divide into {n_kv} key/value heads")
+    fmt = _q8(pages, n_kv, head_dim, what)
+    if q.numel() != tokens * n_heads * head_dim or out.numel() != q.numel() or out.dtype != q.dtype:
+        raise KernelError(f"{what}: q and out must be [tokens, {n_heads}, {head_dim}] of one type")
+    if cu_seqlens.numel() != rows + 1:
+        raise KernelError(f"{what}: cu_seqlens must have one entry more than there are rows")
+    if window < 0 or ring < 0 or ring % PAGE != 0 or (ring > 0 and (window == 0 or max_row_tokens > ring - window + 1)):
+        raise KernelError(f"{what}: a ring of {ring} positions does not hold what a window of {window} and "
+                          f"{max_row_tokens} new tokens see")
+    if not math.isfinite(scale):
+        raise KernelError(f"{what}: the scale must be finite")
+    _table(page_table, table_stride, rows, what)
+    _same_device(what, q, *pages, cu_seqlens, seq_end, page_table, out, status)
+    if tokens == 0 or rows == 0:
+        return
+    span = int(max_end)
+    if window > 0:                    # from a page's border on
+        span = min(span, window + int(max_row_tokens) + PAGE - 1)
+    chunk, n_splits = attention_q8_plan(rows, int(max_row_tokens), span, n_heads, n_kv, head_dim, q.dtype)
+    partial = None
+    if n_splits > 1:
+        partial = torch.empty(tokens * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
+    _check(_lib("attention_q8").mf_attention_q8(
+        _ptr(q, "q"), _ptr(pages.k, "keys"), _ptr(pages.v, "values"), _ptr(pages.k_scale, "key scales"),
+        _ptr(pages.v_scale, "value scales"), _i32(cu_seqlens, "cu_seqlens"), _i32(seq_end, "seq_end"),
+        _i32(page_table, "page_table"), int(table_stride), int(ring), pages.k.shape[0], _ptr(out, "out"),
+        _f32(partial, "partial"), tokens, rows, int(max_row_tokens), n_heads, n_kv, head_dim, int(window), chunk,
+        n_splits, float(scale), dtype_code(q.dtype), fmt, _i32(status, "status"), _stream()), what,
+        2 if n_splits > 1 else 1)
 
 
 # ---------------------------------------------------------------------------------------
@@ -2284,3 +2515,51 @@ def sample(logits: torch.Tensor, out: torch.Tensor, *, temperature: float, top_k
         int(top_k), float(top_p), float(repeat_penalty), float(frequency_penalty),
         float(presence_penalty), int(seed) & 0xFFFFFFFFFFFFFFFF, 1 if update_state else 0,
         _stream()), "sample")
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.Tensor,
+                  draft_logits: Optional[torch.Tensor], accept_u: torch.Tensor, draw_u: torch.Tensor,
+                  temperature: float, accepted: torch.Tensor, tokens: torch.Tensor) -> None:
+    """Drafted tokens held against the target's probabilities.
+
+    Sequence b brings ``n_b = cu_drafts[b+1] - cu_drafts[b]`` drafted tokens (int32 ``drafts``) and n_b + 1 rows
+    of float32 ``logits``, from row ``cu_drafts[b] + b`` on: what the target says in the place of each draft, and
+    behind the last.  ``draft_logits`` (a row a draft): what the drafts were drawn from, at the same
+    temperature; None: they were looked up, q(x) = 1.  A draft is accepted while u q(x) < p(x) with its number
+    of ``accept_u``; the sequence's next token then comes from max(0, p - q) of the first that is not, or from
+    the last row's p, as the lowest index whose running sum exceeds ``draw_u[b]`` times the sum.
+    ``temperature`` below 1e-6 is greedy: drafts are accepted while they are their row's first maximum, and
+    nothing but ``logits`` is read.
+
+    ``accepted[b]`` = drafts accepted, ``tokens[b]`` = the token behind them (int32, on the device).  Numbers
+    are in [0, 1).  Logits are those to draw from: a token that top-k, top-p or a grammar rules out has
+    -infinity.  A row with a NaN (or nothing above -infinity, or +infinity unless greedy) is no distribution:
+    its draft is not accepted and the token is -1, which the next step refuses."""
+    what = "verify_drafts"
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise KernelError(f"{what}: logits must be float32 rows, contiguous along the vocabulary")
+    n, rows, vocab = drafts.numel(), draw_u.numel(), logits.shape[1]
+    if draft_logits is not None:
+        if draft_logits.dtype != torch.float32 or draft_logits.shape != (n, vocab) or \
+                (n > 0 and draft_logits.stride(1) != 1):
+            raise KernelError(f"{what}: the drafts' logits must be float32 [{n}, {vocab}]")
+    if logits.shape[0] != n + rows:
+        raise KernelError(f"{what}: {n} drafts of {rows} sequences need {n + rows} rows of logits, "
+                          f"not {logits.shape[0]}")
+    if cu_drafts.numel() != rows + 1 or accept_u.numel() != n or accepted.numel() != rows or tokens.numel() != rows:
+        raise KernelError(f"{what}: sizes do not fit {n} drafts of {rows} sequences")
+    if not (math.isfinite(temperature) and temperature >= 0.0):
+        raise KernelError(f"{what}: temperature must be finite and not negative")
+    _same_device(what, logits, drafts, cu_drafts, draft_logits, accept_u, draw_u, accepted, tokens)
+    if rows == 0:
+        return
+    lib = _lib("drafts")
+    # two numbers for every piece of a row
+    pieces = torch.empty(2 * (logits.shape[0] + (n if draft_logits is not None else 0)) * lib.mf_draft_pieces(vocab),
+                         dtype=torch.float64, device=logits.device)
+    _check(lib.mf_verify_drafts(
+        logits.data_ptr(), logits.stride(0), _i32(drafts, "drafts"), _i32(cu_drafts, "cu_drafts"),
+        None if draft_logits is None else draft_logits.data_ptr(),
+        0 if draft_logits is None else draft_logits.stride(0), _f32(accept_u, "accept_u"), _f32(draw_u, "draw_u"),
+        float(temperature), _i32(accepted, "accepted"), _i32(tokens, "tokens"), pieces.data_ptr(), n, rows, vocab,
+        _stream()), what, 2)

@@ -45,6 +45,9 @@ LIBRARIES = {
     "moe": ("moe.cu", []),
     "retention": ("retention.cu", []),
     "outer_scan": ("outer_scan.cu", []),
+    "cache_q8": ("cache_q8.cu", []),
+    "attention_q8": ("attention_q8.cu", []),
+    "drafts": ("drafts.cu", []),
 }
 
 
