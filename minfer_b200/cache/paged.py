@@ -22,7 +22,8 @@ server slot (src/server/slot.rs:15-32), and has one kind of layer only.  Here:
   parts that ask for it, and for the sampler.
 
 Layout of a group's storage: ``[entry][page][kv_head][64][head_dim]`` for K and for V (V with
-its own last dimension where a mixer asks for values of another width).
+its own last dimension where a mixer asks for values of another width).  A cache in 8 bits keeps
+codes there and, beside them, a float32 scale for every vector: ``[entry][page][kv_head][64]``.
 """
 from __future__ import annotations
 
@@ -41,6 +42,20 @@ class CacheError(RuntimeError):
 
 class OutOfPages(CacheError):
     pass
+
+
+CACHE_DTYPES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+
+
+def cache_dtype_of(value) -> Optional[torch.dtype]:
+    """The 8-bit type that ``value`` names ("e4m3", "int8", or the torch type); None for None: the
+    cache is kept in the activations' type."""
+    if value is None or value in CACHE_DTYPES.values():
+        return value
+    if value in CACHE_DTYPES:
+        return CACHE_DTYPES[value]
+    raise CacheError(f"a cache is kept in the activations' type (None) or in "
+                     f"{' or '.join(CACHE_DTYPES)}, not in {value!r}")
 
 
 def pages_for(n_positions: int) -> int:
@@ -183,6 +198,9 @@ class CacheGroup:
         v_shape = shape[:-1] + (key.value_dim or key.head_dim,)
         # zeros, once: a page's unwritten positions are masked by length but still multiplied
         # by a zero weight in the tensor-core kernels, so they must never hold NaN or Inf
+        self.quantised = dtype in CACHE_DTYPES.values()
+        if self.quantised and (key.shared_values or key.value_dim not in (0, key.head_dim)):
+            raise CacheError("a cache in 8 bits keeps values of the keys' width beside the keys")
         self._guarded = [Guarded(shape, dtype, device, f"keys of cache group {key}")]
         self.k = self._guarded[0].tensor
         if key.shared_values:
@@ -192,6 +210,12 @@ class CacheGroup:
         else:
             self._guarded.append(Guarded(v_shape, dtype, device, f"values of cache group {key}"))
             self.v = self._guarded[1].tensor
+        self.k_scale = self.v_scale = None
+        if self.quantised:
+            for what in ("keys", "values"):
+                self._guarded.append(Guarded(shape[:-1], torch.float32, device,
+                                             f"scales of the {what} of cache group {key}"))
+            self.k_scale, self.v_scale = self._guarded[2].tensor, self._guarded[3].tensor
         self._index = {e: i for i, e in enumerate(self.entries)}
 
     def max_new_positions(self) -> Optional[int]:
@@ -221,6 +245,19 @@ class CacheGroup:
                 self._table = wider
             self._table[slot, len(have) - 1] = have[-1]
 
+    def shrink(self, slot: int, length: int) -> None:
+        """Gives back the pages that a sequence of ``length`` positions does not need."""
+        have = self.pages[slot]
+        for i in range(len(have) - 1, self.pages_needed(length) - 1, -1):
+            self.pool.give_back(have.pop(), slot)
+            self._table[slot, i] = -1
+
+    def keeps(self, end: int, length: int) -> bool:
+        """Whether a sequence of ``end`` positions still has what one that goes on from ``length`` sees: a
+        ring has written over the positions below ``end - ring``."""
+        first = max(0, length - self.key.window + 1)
+        return not self.ring or first >= length or first >= end - self.ring
+
     def release(self, slot: int) -> None:
         for p in self.pages[slot]:
             self.pool.give_back(p, slot)
@@ -230,6 +267,13 @@ class CacheGroup:
     def entry_tensors(self, entry: int) -> Tuple[torch.Tensor, torch.Tensor]:
         i = self._index[entry]
         return self.k[i], self.v[i]
+
+    def entry_scales(self, entry: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """The scales of an entry's keys and values (None, None unless the cache is in 8 bits)."""
+        if not self.quantised:
+            return None, None
+        i = self._index[entry]
+        return self.k_scale[i], self.v_scale[i]
 
     def table_rows(self, slots: Sequence[int], width: int) -> List[List[int]]:
         rows = []
@@ -282,7 +326,8 @@ class StatePool:
 
 class Cache:
     """Slots, groups and state together.  ``requests`` maps a cache entry to the
-    ``GroupKey`` of the mixer that writes it."""
+    ``GroupKey`` of the mixer that writes it; ``dtype``: the activations' type, or one of
+    ``CACHE_DTYPES`` for keys and values in 8 bits."""
 
     def __init__(self, requests: Dict[int, GroupKey], max_tokens: int, max_seqs: int,
                  dtype: torch.dtype, device: torch.device | str, step_tokens: int = 1):
@@ -338,6 +383,19 @@ class Cache:
         self.slots.check(slot)
         self.slots.length[slot] = length
 
+    def rewind(self, slot: int, length: int) -> None:
+        """Takes a sequence back to its first ``length`` positions."""
+        self.slots.check(slot)
+        end = self.slots.length[slot]
+        if not 0 <= length <= end:
+            raise CacheError(f"a sequence of {end} positions cannot be taken back to {length}")
+        if not all(g.keeps(end, length) for g in self.groups):
+            raise CacheError(f"a ring of the cache no longer holds what a sequence taken back from {end} to "
+                             f"{length} positions would see")
+        for g in self.groups:
+            g.shrink(slot, length)
+        self.slots.length[slot] = length
+
     def max_new_positions(self) -> Optional[int]:
         """Most tokens a sequence may bring in one step that attends over the cache (None: no
         bound): the smallest bound of the groups."""
@@ -354,8 +412,9 @@ class Cache:
 
     def bytes(self) -> int:
         """Bytes of key/value storage that sequences can hold (the spare pages not counted)."""
-        return sum((g.k[:, :g.n_pages].numel() + (0 if g.key.shared_values else g.v[:, :g.n_pages].numel()))
-                   * g.k.element_size() for g in self.groups)
+        codes = sum((g.k[:, :g.n_pages].numel() + (0 if g.key.shared_values else g.v[:, :g.n_pages].numel()))
+                    * g.k.element_size() for g in self.groups)
+        return codes + sum(2 * g.k_scale[:, :g.n_pages].numel() * 4 for g in self.groups if g.quantised)
 
     def free_pages(self) -> List[int]:
         return [g.pool.n_free() for g in self.groups]

@@ -45,6 +45,7 @@ OPTIONS:
   --seed <N>              RNG seed for sampling (default 42)
   --n-ctx <N>             context per sequence (default 4096); sizes the cache
   --dtype <D>             bfloat16 (default) or float32 (true 32-bit everywhere)
+  --cache-dtype <D>       keys and values in the activations' type (default: auto) or in 8 bits: e4m3 or int8
   --no-cuda-graph         launch decode steps kernel by kernel
   -h, --help              show this help
   -V, --version           print version and exit
@@ -71,7 +72,7 @@ def parse_args(argv: List[str]) -> dict:
     opts = {"model": None, "prompt": None, "prompt_file": None, "meta": False, "temp": 0.8,
             "top_k": 40, "top_p": 0.95, "repeat_penalty": 1.1, "frequency_penalty": 0.0,
             "presence_penalty": 0.0, "stop": [], "n_predict": 512, "seed": 42, "n_ctx": 4096,
-            "dtype": "bfloat16", "cuda_graph": True, "command": "run", "store_dtype": "bfloat16",
+            "dtype": "bfloat16", "cache_dtype": None, "cuda_graph": True, "command": "run", "store_dtype": "bfloat16",
             "positional": []}
     i = 0
 
@@ -131,6 +132,12 @@ def parse_args(argv: List[str]) -> dict:
             opts["dtype"] = value(a)
             if opts["dtype"] not in ("bfloat16", "float32", "bf16", "fp32"):
                 raise CliError("--dtype is bfloat16 or float32")
+        elif a == "--cache-dtype":
+            opts["cache_dtype"] = value(a)
+            if opts["cache_dtype"] not in ("auto", "e4m3", "int8"):
+                raise CliError("--cache-dtype is auto, e4m3 or int8")
+            if opts["cache_dtype"] == "auto":
+                opts["cache_dtype"] = None
         elif a == "--store-dtype":
             opts["store_dtype"] = value(a)
         elif a == "--no-cuda-graph":
@@ -247,7 +254,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     if opts.get("max_seqs"):
         batch = max(1, min(batch, opts["max_seqs"]))
     gen = Generator(model, max_tokens=per_seq * batch, max_batch=batch,
-                    cuda_graphs=opts["cuda_graph"])
+                    cuda_graphs=opts["cuda_graph"], cache_dtype=opts["cache_dtype"])
     sampling = SamplingParams(opts["temp"], opts["top_k"], opts["top_p"], opts["repeat_penalty"],
                               opts["frequency_penalty"], opts["presence_penalty"], opts["seed"])
     n_prompt = sum(len(p) for p in prompts)

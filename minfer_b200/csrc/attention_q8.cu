@@ -571,11 +571,15 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
 // the unnormalised output; a split without a visible key has a maximum of -infinity and no output.
 // ------------------------------------------------------------------------------------------
 template <typename T>
-__global__ void attention_q8_merge_kernel(const float* partial, T* __restrict__ out, int n_splits, int hd) {
+__global__ void attention_q8_merge_kernel(const float* partial, T* __restrict__ out, int n_splits, int hd, int n_heads,
+                                          const int* cu_seqlens, int n_rows) {
     pdl_prologue();
     extern __shared__ float mq_s[];                        // [n_splits] factors
     __shared__ float red_s[33];
     const size_t th = blockIdx.x;
+    // tokens of no row stay as they are
+    const int token = blockIdx.x / n_heads;
+    if (token < cu_seqlens[0] || token >= cu_seqlens[n_rows]) return;
     const float* p = partial + th * n_splits * (hd + 2);
     float m = AQ_NEG;
     for (int s = threadIdx.x; s < n_splits; s += blockDim.x) m = fmaxf(m, p[(size_t)s * (hd + 2)]);
@@ -717,9 +721,9 @@ extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v
     if ((long long)n_tokens * n_heads > 0x7fffffffLL) return MF_ERR_UNSUPPORTED;
     if (dtype == MF_DTYPE_F32)
         mf_launch(attention_q8_merge_kernel<float>, dim3((unsigned)(n_tokens * n_heads)), dim3(threads),
-                  (size_t)n_splits * 4, stream, partial, (float*)out, n_splits, hd);
+                  (size_t)n_splits * 4, stream, partial, (float*)out, n_splits, hd, n_heads, cu_seqlens, n_rows);
     else
         mf_launch(attention_q8_merge_kernel<__nv_bfloat16>, dim3((unsigned)(n_tokens * n_heads)), dim3(threads),
-                  (size_t)n_splits * 4, stream, partial, (__nv_bfloat16*)out, n_splits, hd);
+                  (size_t)n_splits * 4, stream, partial, (__nv_bfloat16*)out, n_splits, hd, n_heads, cu_seqlens, n_rows);
     return MF_LAUNCH_CHECK();
 }

@@ -240,15 +240,17 @@ class Generator:
         gen = Generator(Model.from_folder(folder, "bfloat16"), max_tokens=8 * 4096)
         results = gen.generate([[1, 2, 3], [4, 5]], max_new_tokens=32,
                                sampling=SamplingParams.greedy())
+
+    ``cache_dtype``: "e4m3" or "int8" for keys and values in 8 bits (``Engine``).
     """
 
     def __init__(self, model, max_tokens: int = 16384, max_batch: int = 64,
-                 cuda_graphs: bool = True, pipelined: bool = True):
+                 cuda_graphs: bool = True, pipelined: bool = True, cache_dtype=None):
         from .step import Engine
         self.model = model
         self.max_batch = int(max_batch)
         self.engine = Engine(model, max_tokens=max_tokens, max_seqs=max(self.max_batch, 1),
-                             cuda_graphs=cuda_graphs)
+                             cuda_graphs=cuda_graphs, cache_dtype=cache_dtype)
         self.max_tokens = self.engine.cache.max_tokens
         self.stats = GenerationStats()
         self.pipelined = bool(pipelined)    # host one step behind the device (same tokens)
@@ -285,10 +287,11 @@ class Generator:
 def generate(model_or_folder: Any, prompts: Sequence[Sequence[int]], max_new_tokens: int = 512,
              sampling: Optional[SamplingParams] = None,
              stop_token_ids: Optional[Sequence[int]] = None, dtype: str = "bfloat16",
-             max_tokens: Optional[int] = None) -> List[GenerationResult]:
+             max_tokens: Optional[int] = None, cache_dtype=None) -> List[GenerationResult]:
     """The Python entry point: token ids in, token ids out.
 
-    ``model_or_folder`` is a ``Model`` or a folder with config.json and model.safetensors.
+    ``model_or_folder`` is a ``Model`` or a folder with config.json and model.safetensors;
+    ``cache_dtype``: "e4m3" or "int8" for keys and values in 8 bits.
     """
     from ..model import Model
     model = model_or_folder if isinstance(model_or_folder, Model) \
@@ -296,5 +299,6 @@ def generate(model_or_folder: Any, prompts: Sequence[Sequence[int]], max_new_tok
     if max_tokens is None:
         per = max(len(p) for p in prompts) + max_new_tokens
         max_tokens = min(len(prompts), 64) * (((per + PAGE - 1) // PAGE) * PAGE)
-    gen = Generator(model, max_tokens=max_tokens, max_batch=min(max(len(prompts), 1), 64))
+    gen = Generator(model, max_tokens=max_tokens, max_batch=min(max(len(prompts), 1), 64),
+                    cache_dtype=cache_dtype)
     return gen.generate(prompts, max_new_tokens, sampling, stop_token_ids)

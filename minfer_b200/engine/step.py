@@ -27,7 +27,7 @@ from typing import Dict, List, Optional, Sequence
 import numpy as np
 import torch
 
-from ..cache.paged import PAGE, Cache, CacheError, GroupKey
+from ..cache.paged import PAGE, Cache, CacheError, GroupKey, cache_dtype_of
 from ..kernels import api as K
 from ..model import Model
 from ..parts.base import CacheView, CallBinding, StepContext, settle_pending
@@ -73,10 +73,12 @@ class Engine:
     time, each sequence's count rounded up to a multiple of 64; it sizes the cache.
     ``ring_step_tokens``: how many tokens a sequence that goes on may bring in one pass over
     layers with a window (their rings are that much longer than the window; longer rows are
-    run in portions of at least that many tokens)."""
+    run in portions of at least that many tokens).  ``cache_dtype``: "e4m3" or "int8" keeps keys and
+    values in 8 bits with a float32 scale a vector (half the bytes of a bfloat16 cache; models all of
+    whose cached mixers take that); None, in the activations' type."""
 
     def __init__(self, model: Model, max_tokens: int, max_seqs: Optional[int] = None,
-                 cuda_graphs: bool = True, ring_step_tokens: int = 256):
+                 cuda_graphs: bool = True, ring_step_tokens: int = 256, cache_dtype=None):
         if model.device is None or model.device.type != "cuda":
             raise StepError("the model's weights must be on a CUDA device (there is no CPU path)")
         self.model = model
@@ -110,7 +112,17 @@ class Engine:
                         f"a call reads cache entry {call.cache} with {want}, but it is written "
                         f"with {requests.get(call.cache)}")
         self._readers = readers
-        self.cache = Cache(requests, max_tokens, self.max_seqs, self.dtype, self.device,
+        try:
+            self.cache_dtype = cache_dtype_of(cache_dtype)
+        except CacheError as e:
+            raise StepError(str(e)) from None
+        if self.cache_dtype is not None:
+            for call in plan.schedule:
+                mixer = model.blocks[call.layer].mixer
+                if mixer.cache_request() is not None and not getattr(mixer, "accepts_8bit_cache", False):
+                    raise StepError(f"layer {call.layer}'s mixer ({type(mixer).__name__}) keeps its cache in the "
+                                    f"activations' type only; cache_dtype must be None for this model")
+        self.cache = Cache(requests, max_tokens, self.max_seqs, self.cache_dtype or self.dtype, self.device,
                            step_tokens=ring_step_tokens)
         # per-sequence state of fixed size, per call
         self._call_state: List[Dict[str, torch.Tensor]] = []
@@ -135,6 +147,8 @@ class Engine:
             for name in p.libraries(self.dtype):
                 if name not in libs:
                     libs.append(name)
+        if self.cache_dtype is not None:
+            libs += ["cache_q8", "attention_q8"]
         build.prebuild(libs)
         # one word for the error bits of this engine's kernels, read back without waiting: after
         # every step it is copied to pinned host memory, and the next step (or check_status)
@@ -165,6 +179,18 @@ class Engine:
 
     def length(self, slot: int) -> int:
         return self.cache.length(slot)
+
+    def rewind(self, slot: int, length: int) -> None:
+        """Takes the sequence in ``slot`` back to its first ``length`` tokens: the next step goes on from
+        there, as if what came behind had never been fed (drafted tokens that were not accepted).  Refused where
+        that cannot be had: layers with a state of fixed size, or a ring that has written over positions
+        the next token would see."""
+        if any(self._call_state):
+            raise StepError("a sequence with per-sequence state (recurrent layers, token shifts) cannot be taken back")
+        try:
+            self.cache.rewind(slot, int(length))
+        except CacheError as e:
+            raise StepError(str(e)) from None
 
     # ---- one step -----------------------------------------------------------------------
     def step(self, slots: Sequence[int], tokens: Sequence[Sequence[int]],
@@ -476,7 +502,9 @@ class Engine:
             if g is not None and self.model.blocks[call.layer].mixer.cache_request() is not None:
                 k, v = g.entry_tensors(call.cache)
                 table, width = tables[id(g)]
-                view = CacheView(k=k, v=v, page_table=table, table_stride=width, ring=g.ring)
+                k_scale, v_scale = g.entry_scales(call.cache)
+                view = CacheView(k=k, v=v, page_table=table, table_stride=width, ring=g.ring,
+                                 k_scale=k_scale, v_scale=v_scale)
             out.append(CallBinding(
                 cache=view, writes_cache=call.writes_cache, entry=call.cache,
                 has_readers=call.writes_cache and self._readers.get(call.cache, 0) > 0,

@@ -163,19 +163,22 @@ class Model:
         """Seeded random weights for a configuration (``from_config`` with its defaults)."""
         return cls.from_config(config, seed, dtype, device)
 
-    def new_session(self, max_seqs: int = 8, max_positions: int = 4096, cuda_graphs: bool = True):
+    def new_session(self, max_seqs: int = 8, max_positions: int = 4096, cuda_graphs: bool = True,
+                    cache_dtype=None):
         """An ``Engine`` over this model: a cache for ``max_seqs`` sequences of up to
-        ``max_positions`` positions; ``acquire`` slots, ``step`` them, ``release`` them."""
+        ``max_positions`` positions; ``acquire`` slots, ``step`` them, ``release`` them.
+        ``cache_dtype``: "e4m3" or "int8" for keys and values in 8 bits."""
         from .engine.step import Engine
         return Engine(self, max_tokens=max_seqs * max_positions, max_seqs=max_seqs,
-                      cuda_graphs=cuda_graphs)
+                      cuda_graphs=cuda_graphs, cache_dtype=cache_dtype)
 
     def generate(self, prompts, max_new_tokens: int = 512, sampling=None, stop_token_ids=None,
-                 max_batch: int = 8, max_positions: int = 4096):
+                 max_batch: int = 8, max_positions: int = 4096, cache_dtype=None):
         """Token ids in, ``GenerationResult``s out; builds a ``Generator`` for this call (keep
         a ``Generator`` yourself to reuse its cache and captured graphs)."""
         from .engine.generate import Generator
-        gen = Generator(self, max_tokens=max_batch * max_positions, max_batch=max_batch)
+        gen = Generator(self, max_tokens=max_batch * max_positions, max_batch=max_batch,
+                        cache_dtype=cache_dtype)
         return gen.generate(prompts, max_new_tokens, sampling, stop_token_ids)
 
     def export_state_dict(self) -> Dict[str, torch.Tensor]:

@@ -75,6 +75,7 @@ def decode_chunks(items: int, max_end: int, tensor_cores: bool = True,
 
 class Attention(Mixer):
     capturable = True      # launches kernels only; safe inside a CUDA graph capture
+    accepts_8bit_cache = True
 
     def libraries(self, dtype: torch.dtype) -> List[str]:
         libs = ["ops", "attention"]
@@ -197,14 +198,22 @@ class Attention(Mixer):
         elif own_kv:
             # whole prompts of a call that reads another call's entry: that call's keys
             k_step, v_step = ctx.extras[("step_kv", binding.entry)]
-        if cache.k.dtype != act:
+        pages = None
+        if cache.k_scale is not None:
+            pages = K.Q8Pages(cache.k, cache.v, cache.k_scale, cache.v_scale)
+        elif cache.k.dtype != act:
             raise K.KernelError("the cache and the activations must share one dtype")
-        K.rope_kvstore(qkv, ctx.positions, ctx.token_row, ctx.seq_end, inv_freq, q,
-                       k_step if write else None, v_step if write else None,
-                       cache.k if write else None, cache.v if write else None,
-                       cache.page_table if write else None, cache.table_stride, cache.ring,
-                       nh, nk, hd, rotary_dim, style, ctx.status, n_partials=n_partials,
-                       bias=qkv_bias)
+        if pages is not None and write:
+            K.rope_kvstore_q8(qkv, ctx.positions, ctx.token_row, ctx.seq_end, inv_freq, q, k_step, v_step,
+                              pages, cache.page_table, cache.table_stride, cache.ring, nh, nk, hd, rotary_dim,
+                              style, ctx.status, n_partials=n_partials, bias=qkv_bias)
+        else:
+            K.rope_kvstore(qkv, ctx.positions, ctx.token_row, ctx.seq_end, inv_freq, q,
+                           k_step if write else None, v_step if write else None,
+                           cache.k if write else None, cache.v if write else None,
+                           cache.page_table if write else None, cache.table_stride, cache.ring,
+                           nh, nk, hd, rotary_dim, style, ctx.status, n_partials=n_partials,
+                           bias=qkv_bias)
 
         o = torch.empty((n, nh * hd), dtype=act, device=dev)
         if own_kv:
@@ -229,6 +238,14 @@ class Attention(Mixer):
                     f"positions with a window of {self.window} takes "
                     f"{cache.ring - self.window + 1} a step (the engine runs longer rows in portions)")
             n_one = int(ctx.extras.get("single_rows", 0))      # rows of one token, first in the batch
+            if pages is not None:
+                # rows of one token and the others have kernels of their own shape
+                if n_one:
+                    self._over_8bit(q[:n_one], o[:n_one], pages, cache, ctx, 0, n_one, 1)
+                if n_one < ctx.n_rows:
+                    self._over_8bit(q, o, pages, cache, ctx, n_one, ctx.n_rows, ctx.max_row_tokens)
+                self._project_out(o, ctx, residual)
+                return
             if (not ctx.single_token and PROMPT_ATTENTION != "mma" and not FORCE_GENERIC_ATTENTION
                     and K.attention_prefill_supported(q, nh, nk, hd)
                     and ctx.n_tokens - n_one >= PAGED_PROMPT_MIN_TOKENS):
@@ -266,6 +283,14 @@ class Attention(Mixer):
                           cache.table_stride, cache.ring, o, partial, nh, nk, hd, self.window,
                           chunk, n_chunks, self.scale, force_generic=FORCE_GENERIC_ATTENTION,
                           status=ctx.status, old_keys_final=final)
+
+    def _over_8bit(self, q: torch.Tensor, o: torch.Tensor, pages: K.Q8Pages, cache, ctx: StepContext,
+                   first: int, last: int, most: int) -> None:
+        """Rows ``first`` .. ``last`` - 1 of the batch over a cache in 8 bits; ``most``: the most tokens of one."""
+        stride = cache.table_stride
+        K.attention_paged_q8(q, pages, ctx.cu_seqlens[first:last + 1], ctx.seq_end[first:last],
+                             cache.page_table[first * stride:], stride, cache.ring, o, most, ctx.max_end,
+                             self.n_heads, self.n_kv_heads, self.head_dim, self.window, self.scale, ctx.status)
 
     def _project_out(self, o: torch.Tensor, ctx: StepContext, residual: torch.Tensor) -> None:
         target = ctx.extras.pop("prepare_for", None)

@@ -59,6 +59,8 @@ class CacheView:
     page_table: torch.Tensor        # int32 [batch rows, table_stride]
     table_stride: int
     ring: int                       # 0 = linear, else ring length in positions
+    k_scale: Optional[torch.Tensor] = None      # float32 [pages, n_kv_heads, 64]: k and v are 8-bit codes
+    v_scale: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -225,6 +227,8 @@ class Mixer(Part):
     # ``ctx.extras["prepare_for"]`` (a norm), if set, may be answered with a ``Prepared`` in
     # ``ctx.extras["prepared"]`` by the product that adds into the residual
     accepts_row_scale = False
+    # True: the mixer writes and reads cache entries in 8 bits too (``CacheView.k_scale`` set)
+    accepts_8bit_cache = False
 
     def cache_request(self) -> Optional[CacheRequest]:
         return None

@@ -209,6 +209,25 @@ def test_rows_that_see_nothing_and_rows_of_no_tokens(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float32, 64)])
+def test_tokens_of_other_rows_are_left_alone_where_keys_are_split(dtype, dim):
+    """A call over some rows of a step: tokens in front of the first and behind the last stay as they are."""
+    heads, kv, fmt = 4, 2, torch.int8
+    gen, rng = torch.Generator().manual_seed(1), np.random.RandomState(2)
+    ends, cu = [2000, 1500], [2, 3, 5]
+    table, n_pages = make_table(ends, 0, rng)
+    pages = make_pages(table, n_pages, ends, 0, kv, dim, fmt, gen)
+    q = torch.randn(8, heads, dim, generator=gen).to(dtype).to(DEV)
+    assert K.attention_q8_plan(2, 2, 2000, heads, kv, dim, dtype)[1] > 1
+    out = torch.full_like(q, 7.0)
+    K.attention_paged_q8(q, pages, ints(cu), ints(ends), ints(table), len(table[0]), 0, out, 2, 2000, heads, kv, dim, 0,
+                         0.2, status_word())
+    assert (out[:2] == 7.0).all() and (out[5:] == 7.0).all()
+    want, *sizes = plain.attention(q, pages, cu, ends, table, 0, heads, kv, 0, 0.2)
+    tol = plain.attention_tolerance(want, *sizes, dtype, dim, fmt)
+    assert ((out.double().cpu() - want).abs() <= tol)[2:5].all()
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float32, 64)])
 def test_a_page_that_is_not_there_is_not_read(dtype, dim):
     heads, kv, fmt = 4, 2, torch.int8
     gen, rng = torch.Generator().manual_seed(1), np.random.RandomState(2)
