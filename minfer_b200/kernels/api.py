@@ -400,8 +400,9 @@ def _sig_cache_q8(lib: ctypes.CDLL) -> None:
 
 
 def _sig_attention_q8(lib: ctypes.CDLL) -> None:
-    lib.mf_attention_q8_plan.argtypes = [c_int] * 7 + [c_void_p, c_void_p]
-    lib.mf_attention_q8.argtypes = ([c_void_p] * 8 + [c_int] * 3 + [c_void_p, c_void_p] + [c_int] * 9 +
+    lib.mf_attention_q8_plan.argtypes = [c_int] * 7
+    lib.mf_attention_q8_merges.argtypes = [c_int] * 3
+    lib.mf_attention_q8.argtypes = ([c_void_p] * 8 + [c_int] * 3 + [c_void_p, c_void_p] + [c_int] * 8 +
                                     [c_float, c_int, c_int, c_void_p, c_void_p])
 
 
@@ -1231,17 +1232,15 @@ _Q8_PLANS: Dict[tuple, tuple] = {}
 
 
 def attention_q8_plan(n_rows: int, max_row_tokens: int, span: int, n_heads: int, n_kv: int, head_dim: int,
-                      dtype: torch.dtype) -> tuple[int, int]:
-    """(keys of a split, splits) of attention over 8-bit pages; ``span``: the most positions that the queries
-    of a row see."""
+                      dtype: torch.dtype) -> tuple[int, bool]:
+    """(parts that a row's keys are split into, whether a second kernel joins them) of attention over 8-bit
+    pages; ``span``: the most positions that the queries of a row see."""
     key = (torch.cuda.current_device(), n_rows, max_row_tokens, span, n_heads, n_kv, head_dim, dtype)
     got = _Q8_PLANS.get(key)
     if got is None:
-        chunk, splits = c_int(0), c_int(0)
-        _check(_lib("attention_q8").mf_attention_q8_plan(n_rows, max_row_tokens, span, n_heads, n_kv, head_dim,
-                                                         dtype_code(dtype), ctypes.addressof(chunk),
-                                                         ctypes.addressof(splits)), "attention_q8_plan", 0)
-        got = (chunk.value, splits.value)
+        lib, code = _lib("attention_q8"), dtype_code(dtype)
+        splits = lib.mf_attention_q8_plan(n_rows, max_row_tokens, span, n_heads, n_kv, head_dim, code)
+        got = (splits, bool(lib.mf_attention_q8_merges(splits, head_dim, code)))
         if len(_Q8_PLANS) > 4096:
             _Q8_PLANS.clear()
         _Q8_PLANS[key] = got
@@ -1279,17 +1278,17 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
     span = int(max_end)
     if window > 0:                    # from a page's border on
         span = min(span, window + int(max_row_tokens) + PAGE - 1)
-    chunk, n_splits = attention_q8_plan(rows, int(max_row_tokens), span, n_heads, n_kv, head_dim, q.dtype)
+    n_splits, merges = attention_q8_plan(rows, int(max_row_tokens), span, n_heads, n_kv, head_dim, q.dtype)
     partial = None
-    if n_splits > 1:
+    if merges:
         partial = torch.empty(tokens * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
     _check(_lib("attention_q8").mf_attention_q8(
         _ptr(q, "q"), _ptr(pages.k, "keys"), _ptr(pages.v, "values"), _ptr(pages.k_scale, "key scales"),
         _ptr(pages.v_scale, "value scales"), _i32(cu_seqlens, "cu_seqlens"), _i32(seq_end, "seq_end"),
         _i32(page_table, "page_table"), int(table_stride), int(ring), pages.k.shape[0], _ptr(out, "out"),
-        _f32(partial, "partial"), tokens, rows, int(max_row_tokens), n_heads, n_kv, head_dim, int(window), chunk,
+        _f32(partial, "partial"), tokens, rows, int(max_row_tokens), n_heads, n_kv, head_dim, int(window),
         n_splits, float(scale), dtype_code(q.dtype), fmt, _i32(status, "status"), _stream()), what,
-        2 if n_splits > 1 else 1)
+        2 if merges else 1)
 
 
 # ---------------------------------------------------------------------------------------
