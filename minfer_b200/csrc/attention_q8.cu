@@ -13,6 +13,7 @@
 #include "q8.cuh"
 
 #include <cooperative_groups.h>
+#include <type_traits>
 
 struct AttnQ8Args {
     const void* q;                 // [tokens][n_heads][hd]
@@ -25,10 +26,10 @@ struct AttnQ8Args {
     const int* page_table;
     int table_stride, ring, n_pages;
     void* out;                     // [tokens][n_heads][hd]
-    float* partial;                // [tokens][n_heads][n_splits][hd + 2] where n_splits > 1
-    int n_tokens, n_heads, n_kv, hd, window;
+    float* partial;                // scratch, see the kernels
+    int n_tokens, n_rows, n_heads, n_kv, hd, window;
     int n_splits;                  // parts that a row's pages are shared out to
-    int q_groups;                  // blocks along a row's matrix rows
+    int q_groups;                  // blocks along the longest row's matrix rows
     float scale;
     unsigned* status;
 };
@@ -78,19 +79,19 @@ __device__ __forceinline__ float lds32(uint32_t at) {
 // are the 16 rows of a tile and matrix rows its 8 columns.  A group of seven heads then wastes one column in
 // eight, where as rows it would waste nine in sixteen, and a warp holds half the registers.
 //
-// A warp owns 16 keys of every page of its block's split (four warps, 64 positions a page) and streams
+// A warp owns KT * 16 neighbouring keys of every KT pages of its block's split (four warps) and streams
 // them through a ring of its own in shared memory, filled by cp.async: no barrier between warps until
 // the end, where the four results are joined.  An 8-bit code is an exact half, so both products run on
-// halves: a query's row is brought to [2^14, 2^15) by a power of two first (a half has more mantissa
-// than a bfloat16, and 2^-28 of a row's largest element is still exact), the power goes into the
-// float32 factor of its scores.
+// halves: the block's queries are brought below 2^15 by one power of two first (a half has more mantissa
+// than a bfloat16, and 2^-28 of their largest element is still exact), the power goes into the
+// float32 factor of the scores.
 //
-// Values' scales differ from key to key, and a half holds 2^-14..2^16: so beside the reference m of its
-// scores a row carries a reference w of its weights p_j vs_j, and what is rounded to halves is p_j vs_j / w
-// (off by 2^-11, where a bfloat16 probability is off by 2^-8).  Both references are maxima of what came
-// before, moved up (and outputs rescaled) only when a score passes m by more than 8 powers of two or a
-// weight passes w by more than 10: nothing is near overflow until then, sums are float32, and the usual
-// step needs one vote and no exchange between lanes.
+// Values' scales differ from key to key, and a half holds 2^-14..2^16: so what a row's exponentials are
+// taken against is not its largest score but the largest weight so far, m = max_j (s_j + log2 vs_j), and what
+// is rounded to halves is 2^(s_j - m) vs_j (off by 2^-11, where a bfloat16 probability is off by 2^-8); the sum
+// of 2^(s_j - m) is float32.  m is moved up (and outputs rescaled) only when a weight passes it by more than
+// 2^10: nothing is near overflow until then, and the usual step needs one vote and no exchange between
+// lanes.
 //
 // Layouts: row r of a score tile is key 4 (r' >> 1) + 2 (r >> 3) + (r & 1), r' = r & 7, of the step's 16, so that
 // the keys a thread multiplies values of are the four from 4 t on.  Both operands of a score see the same
@@ -99,10 +100,10 @@ __device__ __forceinline__ float lds32(uint32_t at) {
 // ------------------------------------------------------------------------------------------
 #define AQ_WARPS 4
 #define AQ_KEYS 16
-#define AQ_SCORE_ROOM 8.0f        // powers of two
-#define AQ_WEIGHT_ROOM 1024.0f
+#define AQ_WEIGHT_ROOM 1024.0f    // a weight beyond it moves the reference
+#define AQ_SCORE_ROOM 100.0f      // so does 2^100 without a value's scale (which may be zero)
 
-template <int HD> struct AqTile {
+template <int HD> struct AqTile {                          // 16 keys: K, V, scales
     static constexpr int CPR = HD / 16;                    // 16-byte chunks a vector
     static constexpr int CODES = AQ_KEYS * HD;             // bytes of codes, K or V
     static constexpr int STAGE = 2 * CODES + 2 * AQ_KEYS * 4;
@@ -119,16 +120,56 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {          // an 8 x 
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+#define AQ_WHOLE 0
+#define AQ_SPLIT 1
+#define AQ_SHARED 2
+#define AQ_LEAST_PAGES 2          // that a block of AQ_SHARED takes
+
+// What a row of the batch asks for: its tokens and pages, and how many pages all its items have.
+struct AqRow {
+    int tok0, count, end, base0, pages, items;
+};
+__device__ __forceinline__ AqRow aq_row(const AttnQ8Args& a, int b, int rows_a_block) {
+    AqRow r;
+    r.tok0 = a.cu_seqlens[b];
+    r.count = a.cu_seqlens[b + 1] - r.tok0;
+    r.end = a.seq_end[b];
+    if (r.count <= 0 || r.tok0 < 0 || r.tok0 + r.count > a.n_tokens) r.count = 0;
+    const int first = r.end - r.count;
+    r.base0 = (a.window > 0 ? max(0, first - a.window + 1) : 0) & ~(MF_PAGE - 1);
+    r.items = a.n_kv * min(a.q_groups, (r.count * (a.n_heads / a.n_kv) + rows_a_block - 1) / rows_a_block);
+    // (a row that sees nothing still has zeros to write: one page, which no key of it is in)
+    r.pages = r.count > 0 ? max(1, (r.end - r.base0 + MF_PAGE - 1) / MF_PAGE) : 0;
+    return r;
+}
+// AQ_SHARED: block c of n takes pages [c s, (c + 1) s) of all U, s = ceil(U / n).
+__device__ __forceinline__ int aq_share(int units, int blocks) {
+    return max(AQ_LEAST_PAGES, (units + blocks - 1) / blocks);
+}
+// Its scratch: for every block where its first page lies and s, then two results a block (of an item begun by
+// another block, and of one begun here that another ends): [rows][HD] outputs, then maxima and sums.
+struct __align__(16) AqFirst {
+    int row, item, page0, share;               // share 0: the block has no pages
+};
+__host__ __device__ constexpr size_t aq_slot_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
+__host__ __device__ constexpr size_t aq_table_floats(int blocks) { return (size_t)blocks * 4; }
+
 __device__ __forceinline__ float over_keys_max(float v) {             // over the eight lanes of one t
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
     return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
 
-// NT: tiles of 8 matrix rows a block takes.  CLUSTER: the splits of a row are the blocks of a cluster, which
-// join their results through distributed shared memory; else each leaves a partial result for
-// attention_q8_merge_kernel.
-template <int HD, int FMT, int NT, bool CLUSTER, int STAGES, int MINB>
+// NT: tiles of 8 matrix rows a block takes; KT: tiles of 16 keys a warp takes at a time.  An item is one
+// (row of the batch, key/value head, 8 NT matrix rows).  How items are shared out:
+//   AQ_WHOLE    a block an item
+//   AQ_SPLIT    an item's pages are split among the blocks of a cluster, which join their results through
+//               distributed shared memory: one launch, for calls whose blocks are all on the GPU at once
+//   AQ_SHARED   the pages of all items, one behind the other, are dealt out evenly to as many blocks as the
+//               GPU holds, wherever one item ends and the next begins; items that several blocks have
+//               worked on are joined by attention_q8_join_kernel.  Rows of any lengths keep every SM busy
+//               to the end.
+template <int HD, int FMT, int NT, int KT, int MODE, int STAGES, int MINB>
 __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(AttnQ8Args a) {
     using T = AqTile<HD>;
     namespace cg = cooperative_groups;
@@ -136,66 +177,148 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
     constexpr int OS = HD + 4;                             // floats a row of the joining buffer
     constexpr int ROWS = 8 * NT;
     extern __shared__ __align__(128) uint8_t aq_smem[];
-    __shared__ float ml_s[AQ_WARPS][ROWS][3];
+    __shared__ float2 ml_s[AQ_WARPS][ROWS];
     __shared__ float f_s[AQ_WARPS][ROWS];
     __shared__ float2 row_s[ROWS];                         // the block's maximum and sum of each row
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x, hk = blockIdx.y / a.q_groups, qg = blockIdx.y - hk * a.q_groups, b = blockIdx.z;
     const int G = a.n_heads / a.n_kv;
-    const int tok0 = a.cu_seqlens[b], count = a.cu_seqlens[b + 1] - tok0, end = a.seq_end[b];
+
+    // ---- which pages of which items ----
+    int b = blockIdx.z, item = blockIdx.y, page0 = 0, page1 = 0;          // pages [page0, page1) of the item
+    int todo = 0;                                                         // AQ_SHARED: pages left to this block
+    AqFirst first_of;
+    AqRow row;
+    if constexpr (MODE == AQ_SHARED) {
+        // the pages in front of every row and in all, then the row that the block's first page belongs to
+        __shared__ int scan_s[AQ_WARPS], at_s[2];
+        int units = 0, before = 0, share = 0, begin = 0;
+        for (int b0 = 0; b0 < a.n_rows;) {
+            int mine = 0;
+            if (b0 + tid < a.n_rows) {
+                const AqRow r = aq_row(a, b0 + tid, ROWS);
+                mine = r.pages * r.items;
+            }
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            __syncthreads();
+            if (lane == 31) scan_s[warp] = upto;
+            __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int w = 0; w < AQ_WARPS; ++w) {
+                if (w < warp) upto += scan_s[w];
+                all += scan_s[w];
+            }
+            const bool known = share > 0;                                 // (the second time through)
+            if (!known) units += all;
+            const bool done = !known && b0 + AQ_WARPS * 32 >= a.n_rows;
+            if (done) {
+                share = aq_share(units, gridDim.x);
+                begin = blockIdx.x * share;
+                todo = min(share, units - begin);
+            }
+            if (known || a.n_rows <= AQ_WARPS * 32) {
+                const int from = before + upto - mine;
+                if (mine > 0 && from <= begin && begin < from + mine) { at_s[0] = b0 + tid; at_s[1] = from; }
+                before += all;
+            }
+            b0 += AQ_WARPS * 32;
+            if (done && a.n_rows > AQ_WARPS * 32 && todo > 0) b0 = 0;     // once more, with the block's page known
+        }
+        __syncthreads();
+        AqFirst* firsts = (AqFirst*)a.partial;
+        if (todo <= 0) {
+            // (what a kernel before this one may still read of its own scratch is not touched before it has ended)
+            pdl_wait();
+            if (tid == 0) firsts[blockIdx.x].share = 0;
+            return;
+        }
+        b = at_s[0];
+        row = aq_row(a, b, ROWS);
+        item = (begin - at_s[1]) / row.pages;
+        page0 = begin - at_s[1] - item * row.pages;
+        first_of.row = b; first_of.item = item; first_of.page0 = page0; first_of.share = share;
+    } else {
+        row = aq_row(a, b, ROWS);
+        // (uniform over a cluster)
+        if (item >= row.items) { pdl_wait(); return; }
+        const int chunk = MODE == AQ_SPLIT ? (row.pages + a.n_splits - 1) / a.n_splits : row.pages;
+        page0 = min(row.pages, (int)blockIdx.x * chunk);
+        page1 = min(row.pages, page0 + chunk);
+    }
+    bool waited = false;
+
+    for (;;) {
+    if constexpr (MODE == AQ_SHARED) page1 = min(row.pages, page0 + todo);
+    const int tok0 = row.tok0, count = row.count, end = row.end;
+    const int hk = item % a.n_kv, qg = item / a.n_kv;
     const int r0 = qg * ROWS, rows = min(ROWS, count * G - r0);           // the block's matrix rows
-    // (uniform over a cluster)
-    if (rows <= 0 || tok0 < 0 || tok0 + count > a.n_tokens) { pdl_wait(); return; }
     // what the block's queries see together: [lo, hi); and every one of them: [lo_in, hi_in)
     const int first = end - count + r0 / G, last = end - count + (r0 + rows - 1) / G;
     const int lo_all = a.window > 0 ? max(0, first - a.window + 1) : 0;
     const int lo_in = a.window > 0 ? max(0, last - a.window + 1) : 0, hi_in = first + 1;
-    // the row's own pages, shared out evenly
-    const int base0 = lo_all & ~(MF_PAGE - 1), pages = max(0, (last - base0 + MF_PAGE) / MF_PAGE);
-    const int chunk = (pages + a.n_splits - 1) / a.n_splits * MF_PAGE;
-    const int base = base0 + split * chunk;
-    const int lo = max(lo_all, base), hi = min(last + 1, base + chunk);
-    const int n_it = hi > lo ? (hi - base + MF_PAGE - 1) / MF_PAGE : 0;
+    const int base = row.base0 + page0 * MF_PAGE;
+    const int lo = max(lo_all, base), hi = min(last + 1, row.base0 + page1 * MF_PAGE);
+    const int n_it = hi > lo ? (hi - base + KT * MF_PAGE - 1) / (KT * MF_PAGE) : 0;
     const int* table = a.page_table + (size_t)b * a.table_stride;
 
     // ---- the ring ----
-    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(aq_smem) + warp * STAGES * T::STAGE;
+    constexpr int STAGE = KT * T::STAGE;
+    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(aq_smem) + warp * STAGES * STAGE;
+    const int key0 = base + warp * KT * AQ_KEYS;           // the warp's first key of iteration 0
+    const int in_page = key0 & (MF_PAGE - 1);
     int ids = -1;                              // lane i: the page of iteration (it & ~31) + i
+    unsigned there = 0, there_next = 0;        // bit i: so many iterations on, that page is one
     auto look_up = [&](int it) {               // the next 32 page numbers
-        const int p = base + (it + lane) * MF_PAGE;
+        const int p = key0 + (it + lane) * KT * MF_PAGE;
         const int index = (a.ring > 0 ? p % a.ring : p) >> 6;
-        ids = it + lane < n_it && index < a.table_stride ? table[index] : -1;
+        const bool seen = p < hi && p + KT * AQ_KEYS > lo;
+        ids = seen && index < a.table_stride ? table[index] : -1;
+        const bool page = ids >= 0 && ids < a.n_pages;
         // a page that is not there: its keys are seen by nobody, and the caller is told
-        if (it + lane < n_it && (ids < 0 || ids >= a.n_pages)) {
-            ids = -1;
-            if (warp == 0) atomicOr(a.status, MF_STATUS_BAD_POSITION);
-        }
+        if (seen && !page) atomicOr(a.status, MF_STATUS_BAD_POSITION);
+        there_next = __ballot_sync(0xffffffffu, page);
     };
     look_up(0);
-    pdl_wait();
-    unsigned filled = 0;                       // bit it & 31: the iteration's stage holds keys
+    there = there_next;
+    // what a lane copies, from the pages' beginnings on
+    const size_t vectors = (size_t)hk * MF_PAGE + in_page;
+    const uint8_t* const k_from = a.k_codes + vectors * HD + lane * 16;
+    const uint8_t* const v_from = a.v_codes + vectors * HD + lane * 16;
+    const float* const s_from = (lane < 4 ? a.k_scales : a.v_scales - 16) + vectors + lane * 4;
+    const size_t page_vectors = (size_t)a.n_kv * MF_PAGE;
+    const uint32_t k_lane = T::k_at(lane / T::CPR, lane % T::CPR), v_lane = T::CODES + T::v_at(lane / T::CPR, lane % T::CPR);
     uint32_t fetch_to = ring0;
+    if (!waited) {
+        pdl_wait();
+        if (MODE == AQ_SHARED && tid == 0) ((AqFirst*)a.partial)[blockIdx.x] = first_of;
+    }
+    waited = true;
     auto fetch = [&](int it) {
         if ((it & 31) == 0 && it > 0) look_up(it);
-        const int page = __shfl_sync(0xffffffffu, ids, it & 31);
-        const int k0 = base + it * MF_PAGE + warp * AQ_KEYS;
-        const bool here = it < n_it && page >= 0 && k0 < hi && k0 + AQ_KEYS > lo;
-        filled = (filled & ~(1u << (it & 31))) | ((here ? 1u : 0u) << (it & 31));
-        if (here) {
-            const long long at = ((long long)page * a.n_kv + hk) * MF_PAGE + warp * AQ_KEYS;
-            const uint8_t* kp = a.k_codes + at * HD + lane * 16;
-            const uint8_t* vp = a.v_codes + at * HD + lane * 16;
+        if (it < n_it && ((there_next >> (it & 31)) & 1u)) {
+            const size_t at = (size_t)__shfl_sync(0xffffffffu, ids, it & 31) * page_vectors;
+            const uint8_t* kp = k_from + at * HD;
+            const uint8_t* vp = v_from + at * HD;
 #pragma unroll
-            for (int i = 0; i < AQ_KEYS * T::CPR / 32; ++i) {
-                const int u = i * 32 + lane, r = u / T::CPR, c = u % T::CPR;
-                cp16(fetch_to + T::k_at(r, c), kp + i * 512);
-                cp16(fetch_to + T::CODES + T::v_at(r, c), vp + i * 512);
+            for (int k = 0; k < KT; ++k) {
+#pragma unroll
+                for (int i = 0; i < AQ_KEYS * T::CPR / 32; ++i) {
+                    // row lane / CPR + (32 / CPR) i: a multiple of 2 further, so that K's permutation is the
+                    // lane's; V's changes by the rows' quads (stages are multiples of 128 bytes)
+                    constexpr int V_STEP = HD == 128 ? 32 : 64;
+                    cp16(fetch_to + k * T::STAGE + k_lane + i * 512, kp + (k * AQ_KEYS * HD + i * 512));
+                    cp16(((fetch_to + k * T::STAGE + v_lane) ^ (i * V_STEP)) + i * 512, vp + (k * AQ_KEYS * HD + i * 512));
+                }
+                if (lane < 8) cp16(fetch_to + k * T::STAGE + 2 * T::CODES + lane * 16, s_from + at + k * AQ_KEYS);
             }
-            if (lane < 8)
-                cp16(fetch_to + 2 * T::CODES + lane * 16, (lane < 4 ? a.k_scales : a.v_scales - 16) + at + lane * 4);
         }
-        fetch_to = fetch_to == ring0 + (STAGES - 1) * T::STAGE ? ring0 : fetch_to + T::STAGE;
+        fetch_to = fetch_to == ring0 + (STAGES - 1) * STAGE ? ring0 : fetch_to + STAGE;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
@@ -203,89 +326,98 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
 
     // ---- queries: a thread loads a part of row g of each tile; it works on the scores of rows 2 t, 2 t + 1 ----
     uint32_t qb[NT][HD / 16][2];
-    float c_q[NT][2];                          // scale log2(e) / the row's power of two
-    int hi_q[NT][2], lo_q[NT][2];              // positions the row sees: [lo, hi)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int r = n * 8 + g;
-        uint4 w[HD / 64][2];
+    float neg[NT][2];                          // minus the reference: infinity before the first key, NaN for a
+                                               // row that holds what is not finite
+    float c_q;                                 // scale log2(e) / the queries' power of two
+    {
+        uint4 w[NT][HD / 64][2];
         unsigned top = 0;
-        if (r < rows) {
-            const int token = (r0 + r) / G, head = hk * G + (r0 + r) - token * G;
-            const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + ((size_t)(tok0 + token) * a.n_heads + head) * HD;
+        bool bad[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 8 + g;
+            if (r < rows) {
+                const int token = (r0 + r) / G, head = hk * G + (r0 + r) - token * G;
+                const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + ((size_t)(tok0 + token) * a.n_heads + head) * HD;
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) w[n][c][i] = *reinterpret_cast<const uint4*>(q + 64 * c + 16 * t + 8 * i);
+            } else {
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c) w[n][c][0] = w[n][c][1] = make_uint4(0, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            unsigned mine = 0;
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) w[c][i] = *reinterpret_cast<const uint4*>(q + 64 * c + 16 * t + 8 * i);
-        } else {
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t x[4] = {w[n][c][i].x, w[n][c][i].y, w[n][c][i].z, w[n][c][i].w};
 #pragma unroll
-            for (int c = 0; c < HD / 64; ++c) w[c][0] = w[c][1] = make_uint4(0, 0, 0, 0);
+                    for (int j = 0; j < 4; ++j) mine = max(mine, max(x[j] & 0x7fffu, (x[j] >> 16) & 0x7fffu));
+                }
+            mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+            mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+            bad[n] = mine >= 0x7f80u;
+            if (!bad[n]) top = max(top, mine);
         }
-#pragma unroll
-        for (int c = 0; c < HD / 64; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t x[4] = {w[c][i].x, w[c][i].y, w[c][i].z, w[c][i].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = max(top, max(x[j] & 0x7fffu, (x[j] >> 16) & 0x7fffu));
-            }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the power of two: 2^(14 - exponent), from the exponent field (0: a row of zeros or of numbers
-        // below the normal range, which 2^100 brings up and which count as zero below 2^-124)
+        top = __reduce_max_sync(0xffffffffu, top);
+        // the power of two: 2^(14 - exponent), from the exponent field (0: zeros or numbers below the normal
+        // range, which 2^100 brings up and which count as zero below 2^-124)
         const int field = (int)(top >> 7);
         const int power = field == 0 ? 100 : min(141 - field, 100);
         const float up = __int_as_float((power + 127) << 23), down = __int_as_float((127 - power) << 23);
-        const float c_row = field == 255 ? __int_as_float(0x7fc00000) : a.scale * 1.4426950408889634f * down;
+        c_q = a.scale * 1.4426950408889634f * down;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            c_q[n][i] = __shfl_sync(0xffffffffu, c_row, (2 * t + i) * 4);
-            const int rq = n * 8 + 2 * t + i;
-            hi_q[n][i] = rq < rows ? end - count + (r0 + rq) / G + 1 : 0;
-            lo_q[n][i] = rq < rows && a.window > 0 ? max(0, hi_q[n][i] - a.window) : 0;
-        }
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c)
+            for (int i = 0; i < 2; ++i)
+                neg[n][i] = __shfl_sync(0xffffffffu, bad[n] ? __int_as_float(0x7fc00000) : INFINITY, (2 * t + i) * 4);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t x[4] = {w[c][i].x, w[c][i].y, w[c][i].z, w[c][i].w};
+            for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    // a non-finite element makes its row's factor NaN; here it only has to stay finite
-                    const float f0 = field == 255 ? 0.0f : __uint_as_float(x[j] << 16) * up;
-                    const float f1 = field == 255 ? 0.0f : __uint_as_float(x[j] & 0xffff0000u) * up;
-                    // elements 8 i + 2 j, + 1 of the thread's 16: k-step 2 i + j / 2, first or second pair
-                    qb[n][4 * c + 2 * i + (j >> 1)][j & 1] = pack_half2(f0, f1);
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t x[4] = {w[n][c][i].x, w[n][c][i].y, w[n][c][i].z, w[n][c][i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float f0 = bad[n] ? 0.0f : __uint_as_float(x[j] << 16) * up;
+                        const float f1 = bad[n] ? 0.0f : __uint_as_float(x[j] & 0xffff0000u) * up;
+                        // elements 8 i + 2 j, + 1 of the thread's 16: k-step 2 i + j / 2, first or second pair
+                        qb[n][4 * c + 2 * i + (j >> 1)][j & 1] = pack_half2(f0, f1);
+                    }
                 }
-            }
+        }
     }
 
-    // references: neg = -m (infinity before the first key), norm = w, inv = 1 / w
-    float neg[NT][2], l_q[NT][2], norm[NT][2], inv[NT][2], o[NT][OT][4];
+    float l_q[NT][2], o[NT][OT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) { neg[n][i] = INFINITY; l_q[n][i] = norm[n][i] = inv[n][i] = 0.0f; }
+        l_q[n][0] = l_q[n][1] = 0.0f;
 #pragma unroll
         for (int j = 0; j < OT; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
     }
 
     const int key_a = 4 * (g >> 1) + (g & 1);              // the thread's keys: this one and the one 2 behind
+    const uint32_t ka_at = T::k_at(key_a, t), kb_at = T::k_at(key_a + 2, t);
+    const uint32_t v_at0 = T::CODES + (HD == 128 ? T::v_at(4 * t, g) : T::v_at(4 * t, g >> 1) + 8 * (g & 1));
+    const uint32_t s_at = 2 * T::CODES + key_a * 4;
     uint32_t stage = ring0;
-    for (int it = 0; it < n_it; ++it) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-        __syncwarp();
-        if ((filled >> (it & 31)) & 1u) {
-            const int k0 = base + it * MF_PAGE + warp * AQ_KEYS;
-            // ---- scores (two accumulators a tile: half as long a chain) ----
-            float sc[NT][2][4];
+
+    // 16 KT keys from position k0 on.  EDGE: some of them are not seen by some of the rows.
+    auto step = [&](auto edge_tag, int k0) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
+        float sc[KT][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+        for (int k = 0; k < KT; ++k) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) sc[n][h][0] = sc[n][h][1] = sc[n][h][2] = sc[n][h][3] = 0.0f;
+            for (int n = 0; n < NT; ++n) sc[k][n][0] = sc[k][n][1] = sc[k][n][2] = sc[k][n][3] = 0.0f;
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c) {
-                const uint4 ka = lds128(stage + T::k_at(key_a, 4 * c + t)), kb = lds128(stage + T::k_at(key_a + 2, 4 * c + t));
+                // (the second 64 dimensions lie in the other half of 128 bytes)
+                const uint4 ka = lds128((stage + k * T::STAGE + ka_at) ^ (c * 64)), kb = lds128((stage + k * T::STAGE + kb_at) ^ (c * 64));
                 const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -293,114 +425,150 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
                     const uint32_t af[4] = {q8_halves<FMT, false>(x), q8_halves<FMT, false>(y), q8_halves<FMT, true>(x),
                                             q8_halves<FMT, true>(y)};
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_f16(sc[n][j & 1], af, qb[n][4 * c + j][0], qb[n][4 * c + j][1]);
-                }
-            }
-            // values: HD / 8 dimensions of the keys 4 t .. 4 t + 3
-            uint32_t vw[4][HD / 32];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (HD == 128) {
-                    const uint4 x = lds128(stage + T::CODES + T::v_at(4 * t + i, g));
-                    vw[i][0] = x.x; vw[i][1] = x.y; vw[i][2] = x.z; vw[i][3] = x.w;
-                } else {
-                    const uint2 x = lds64(stage + T::CODES + T::v_at(4 * t + i, g >> 1) + 8 * (g & 1));
-                    vw[i][0] = x.x; vw[i][1] = x.y;
-                }
-            }
-            const float ks[2] = {lds32(stage + 2 * T::CODES + key_a * 4), lds32(stage + 2 * T::CODES + key_a * 4 + 8)};
-            const float vs[2] = {lds32(stage + 2 * T::CODES + 64 + key_a * 4), lds32(stage + 2 * T::CODES + 64 + key_a * 4 + 8)};
-            const bool edge = k0 < max(lo_in, lo) || k0 + AQ_KEYS > min(hi_in, hi);       // uniform
-            if (edge) {
-                // codes of places that no query of the block sees are anybody's
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (k0 + 4 * t + i < lo || k0 + 4 * t + i >= hi) {
-#pragma unroll
-                        for (int h = 0; h < HD / 32; ++h) vw[i][h] = 0u;
-                    }
-            }
-            // ---- weights ----
-            uint32_t pb[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float x[2][2], w[2][2];                    // [key][row]
-                unsigned gone = 0;                         // bit 2 k + i: row i does not see key k
-                if (edge)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int at = k0 + key_a + 2 * k;
-                            if (at >= min(hi_q[n][i], hi) || at < max(lo_q[n][i], lo)) gone |= 1u << (2 * k + i);
-                        }
-                auto weigh = [&]() {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float s = sc[n][0][2 * k + i] + sc[n][1][2 * k + i];
-                            x[k][i] = fmaf(s, c_q[n][i] * ks[k], neg[n][i]);
-                            // (a key or value that is not seen may have any scale: NaN must not get in)
-                            if (edge && ((gone >> (2 * k + i)) & 1u)) x[k][i] = AQ_NEG;
-                            const float p = ex2(x[k][i]);
-                            w[k][i] = p * (vs[k] * inv[n][i]);
-                            if (edge && ((gone >> (2 * k + i)) & 1u)) w[k][i] = 0.0f;
-                        }
-                };
-                weigh();
-                const float most = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-                const float heaviest = fmaxf(fmaxf(w[0][0], w[0][1]), fmaxf(w[1][0], w[1][1]));
-                if (__any_sync(0xffffffffu, most > AQ_SCORE_ROOM || heaviest > AQ_WEIGHT_ROOM)) {
-                    // both references up to the maxima that are known now
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float s[2], top = AQ_NEG, big = 0.0f;
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            s[k] = (sc[n][0][2 * k + i] + sc[n][1][2 * k + i]) * (c_q[n][i] * ks[k]);
-                            if ((gone >> (2 * k + i)) & 1u) s[k] = AQ_NEG;
-                            top = fmaxf(top, s[k]);
-                        }
-                        const float before = -neg[n][i], m = fmaxf(before, over_keys_max(top));
-                        const float f = before == AQ_NEG ? 0.0f : ex2(before - m);
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            if (!((gone >> (2 * k + i)) & 1u)) big = fmaxf(big, ex2(s[k] - m) * vs[k]);
-                        const float held = norm[n][i] * f;
-                        big = fmaxf(fmaxf(held, over_keys_max(big)), 7.5e-37f);            // (2^-120: 1 / w is finite)
-                        neg[n][i] = -m;
-                        l_q[n][i] *= f;
-                        norm[n][i] = big;
-                        inv[n][i] = __fdividef(1.0f, big);
-                        const float down = held * inv[n][i];
-#pragma unroll
-                        for (int j = 0; j < OT; ++j) { o[n][j][i] *= down; o[n][j][2 + i] *= down; }
-                    }
-                    weigh();
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) l_q[n][i] += ex2(x[0][i]) + ex2(x[1][i]);
-                pb[n][0] = transposed(pack_half2(w[0][0], w[0][1]));
-                pb[n][1] = transposed(pack_half2(w[1][0], w[1][1]));
-            }
-            // ---- values: pairs of keys of one dimension ----
-#pragma unroll
-            for (int h = 0; h < HD / 32; ++h) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t x = q8_prepare<FMT>(__byte_perm(vw[0][h], vw[1][h], u ? 0x7362 : 0x5140));
-                    const uint32_t y = q8_prepare<FMT>(__byte_perm(vw[2][h], vw[3][h], u ? 0x7362 : 0x5140));
-                    const uint32_t af[4] = {q8_halves<FMT, false>(x), q8_halves<FMT, true>(x), q8_halves<FMT, false>(y),
-                                            q8_halves<FMT, true>(y)};
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * h + u], af, pb[n][0], pb[n][1]);
+                    for (int n = 0; n < NT; ++n) mma_f16(sc[k][n], af, qb[n][4 * c + j][0], qb[n][4 * c + j][1]);
                 }
             }
         }
+        float ks[KT][2], vs[KT][2];
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                ks[k][u] = lds32(stage + k * T::STAGE + s_at + 8 * u) * c_q;
+                vs[k][u] = lds32(stage + k * T::STAGE + s_at + 64 + 8 * u);
+            }
+        // bit 2 u + i of gone[k][n]: row i of tile n does not see key u of tile k
+        unsigned gone[KT][NT];
+        if constexpr (EDGE) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                int to[2], from[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = n * 8 + 2 * t + i, pos = r < rows ? end - count + (r0 + r) / G : -1;
+                    to[i] = min(pos + 1, hi);
+                    from[i] = a.window > 0 ? max(lo, pos - a.window + 1) : lo;
+                }
+#pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    gone[k][n] = 0;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int at = k0 + k * AQ_KEYS + key_a + 2 * u;
+                            if (at >= to[i] || at < from[i]) gone[k][n] |= 1u << (2 * u + i);
+                        }
+                }
+            }
+        }
+        float x[KT][NT][4], w[KT][NT][4];
+        float most = AQ_NEG, heaviest = 0.0f;
+        auto weigh = [&]() {
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {          // 2 key + row
+                        x[k][n][e] = fmaf(sc[k][n][e], ks[k][e >> 1], neg[n][e & 1]);
+                        // (a key or value that is not seen may have any scale: NaN must not get in)
+                        if (EDGE && ((gone[k][n] >> e) & 1u)) x[k][n][e] = AQ_NEG;
+                        w[k][n][e] = ex2(x[k][n][e]) * vs[k][e >> 1];
+                        if (EDGE && ((gone[k][n] >> e) & 1u)) w[k][n][e] = 0.0f;
+                        most = fmaxf(most, x[k][n][e]);
+                        heaviest = fmaxf(heaviest, w[k][n][e]);
+                    }
+        };
+        weigh();
+        if (__any_sync(0xffffffffu, most > AQ_SCORE_ROOM || heaviest > AQ_WEIGHT_ROOM)) {
+            // the references up to what is known now: the largest score first, then the largest weight
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float top = AQ_NEG, big = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            if (!EDGE || !((gone[k][n] >> (2 * u + i)) & 1u)) top = fmaxf(top, sc[k][n][2 * u + i] * ks[k][u]);
+                    const float before = -neg[n][i];
+                    top = over_keys_max(top);
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            if (!EDGE || !((gone[k][n] >> (2 * u + i)) & 1u))
+                                big = fmaxf(big, ex2(fmaf(sc[k][n][2 * u + i], ks[k][u], -top)) * vs[k][u]);
+                    big = fmaxf(over_keys_max(big), 8.1e-28f);         // (2^-90: values of zeros)
+                    // (a row that has seen nothing yet keeps its infinity, one that is NaN its NaN)
+                    const float m = fmaxf(before, top + __log2f(big));
+                    const float f = before == AQ_NEG ? 0.0f : ex2(before - m);
+                    if (top > AQ_NEG && before == before) neg[n][i] = -m;
+                    l_q[n][i] *= f;
+#pragma unroll
+                    for (int j = 0; j < OT; ++j) { o[n][j][i] *= f; o[n][j][2 + i] *= f; }
+                }
+            weigh();
+        }
+        uint32_t pb[KT][NT][2];
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) l_q[n][i] += ex2(x[k][n][i]) + ex2(x[k][n][2 + i]);
+                pb[k][n][0] = transposed(pack_half2(w[k][n][0], w[k][n][1]));
+                pb[k][n][1] = transposed(pack_half2(w[k][n][2], w[k][n][3]));
+            }
+        // ---- values: pairs of keys of one dimension, HD / 8 dimensions of the keys 4 t .. 4 t + 3 ----
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+            uint32_t vw[4][HD / 32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t v0 = stage + k * T::STAGE + v_at0;
+                const uint32_t at = HD == 128 ? v0 + i * 128 : (v0 ^ ((i & 1) * 64)) + (i >> 1) * 128;
+                if constexpr (HD == 128) {
+                    const uint4 v = lds128(at);
+                    vw[i][0] = v.x; vw[i][1] = v.y; vw[i][2] = v.z; vw[i][3] = v.w;
+                } else {
+                    const uint2 v = lds64(at);
+                    vw[i][0] = v.x; vw[i][1] = v.y;
+                }
+                // codes of places that no query of the block sees are anybody's
+                if (EDGE && (k0 + k * AQ_KEYS + 4 * t + i < lo || k0 + k * AQ_KEYS + 4 * t + i >= hi))
+#pragma unroll
+                    for (int h = 0; h < HD / 32; ++h) vw[i][h] = 0u;
+            }
+#pragma unroll
+            for (int h = 0; h < HD / 32; ++h)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t y = q8_prepare<FMT>(__byte_perm(vw[0][h], vw[1][h], u ? 0x7362 : 0x5140));
+                    const uint32_t z = q8_prepare<FMT>(__byte_perm(vw[2][h], vw[3][h], u ? 0x7362 : 0x5140));
+                    const uint32_t af[4] = {q8_halves<FMT, false>(y), q8_halves<FMT, true>(y), q8_halves<FMT, false>(z),
+                                            q8_halves<FMT, true>(z)};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * h + u], af, pb[k][n][0], pb[k][n][1]);
+                }
+        }
+    };
+
+    const int lo_edge = max(lo_in, lo), hi_edge = min(hi_in, hi) - KT * AQ_KEYS;
+    for (int it = 0; it < n_it; ++it) {
+        if ((it & 31) == 0 && it > 0) there = there_next;
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();
+        if ((there >> (it & 31)) & 1u) {
+            const int k0 = key0 + it * KT * MF_PAGE;
+            if (k0 < lo_edge || k0 > hi_edge) step(std::true_type{}, k0);
+            else step(std::false_type{}, k0);
+        }
         __syncwarp();                          // the stage the next fetch fills was read an iteration ago
         fetch(it + STAGES - 1);
-        stage = stage == ring0 + (STAGES - 1) * T::STAGE ? ring0 : stage + T::STAGE;
+        stage = stage == ring0 + (STAGES - 1) * STAGE ? ring0 : stage + STAGE;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
@@ -413,10 +581,9 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
             l += __shfl_xor_sync(0xffffffffu, l, 4);
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
-            if (g == 0) {
-                float* to = ml_s[warp][n * 8 + 2 * t + i];
-                to[0] = -neg[n][i]; to[1] = l; to[2] = norm[n][i];
-            }
+            // (a row that holds what is not finite: its reference is NaN, its sum too)
+            const bool bad = neg[n][i] != neg[n][i];
+            if (g == 0) ml_s[warp][n * 8 + 2 * t + i] = make_float2(bad ? AQ_NEG : -neg[n][i], bad ? neg[n][i] : l);
         }
     __syncthreads();                           // also: every warp is done with its ring
     float* o_s = (float*)aq_smem;
@@ -433,13 +600,13 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
     if (tid < ROWS) {
         float m = AQ_NEG, l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < AQ_WARPS; ++w) m = fmaxf(m, ml_s[w][tid][0]);
+        for (int w = 0; w < AQ_WARPS; ++w) m = fmaxf(m, ml_s[w][tid].x);
         const float m_use = m == AQ_NEG ? 0.0f : m;
 #pragma unroll
         for (int w = 0; w < AQ_WARPS; ++w) {
-            const float f = exp2f(ml_s[w][tid][0] - m_use);
-            f_s[w][tid] = f * ml_s[w][tid][2];
-            l += ml_s[w][tid][1] * f;
+            const float f = exp2f(ml_s[w][tid].x - m_use);
+            f_s[w][tid] = f;
+            l += ml_s[w][tid].y * f;
         }
         row_s[tid] = make_float2(l != l ? INFINITY : m, l);      // NaN among the scores: joining must not pass over it
     }
@@ -464,9 +631,9 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
             make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
     };
     const int units = rows * (HD / 4);
-    if constexpr (CLUSTER) {
+    if constexpr (MODE == AQ_SPLIT) {
         cg::cluster_group cluster = cg::this_cluster();
-        const int n = a.n_splits, rank = split;
+        const int n = a.n_splits, rank = blockIdx.x;
         // the block's own sum over its warps goes where the first warp's was
         for (int i = tid; i < units; i += AQ_WARPS * 32) {
             const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
@@ -501,28 +668,109 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
             write_out(r, d, acc, l == 0.0f ? 0.0f : 1.0f / l);
         }
         cluster.sync();                        // nobody leaves while its memory is read
-    } else if (a.n_splits > 1) {
-        for (int r = tid; r < rows; r += AQ_WARPS * 32) {
-            const int token = (r0 + r) / G, head = hk * G + (r0 + r) - token * G;
-            *reinterpret_cast<float2*>(a.partial + (((size_t)(tok0 + token) * a.n_heads + head) * a.n_splits + split) *
-                                                       (HD + 2)) = row_s[r];
-        }
-        if (n_it == 0) return;                 // no key: the merge reads the maximum only
-        for (int i = tid; i < units; i += AQ_WARPS * 32) {
-            const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
-            const float4 v = joined(r, d);
-            const int token = (r0 + r) / G, head = hk * G + (r0 + r) - token * G;
-            float* p = a.partial + (((size_t)(tok0 + token) * a.n_heads + head) * a.n_splits + split) * (HD + 2) + 2 + d;
-            *reinterpret_cast<float2*>(p) = make_float2(v.x, v.y);
-            *reinterpret_cast<float2*>(p + 2) = make_float2(v.z, v.w);
-        }
+        return;
     } else {
-        for (int i = tid; i < units; i += AQ_WARPS * 32) {
-            const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
-            const float l = row_s[r].y;
-            write_out(r, d, joined(r, d), l == 0.0f ? 0.0f : 1.0f / l);
+        if (MODE == AQ_SHARED && (page0 > 0 || page1 < row.pages)) {
+            // a part of the item: the first result if another block began it, else the second
+            float* slot = a.partial + aq_table_floats(gridDim.x) + (2 * (size_t)blockIdx.x + (page0 > 0 ? 0 : 1)) * aq_slot_floats(ROWS, HD);
+            for (int i = tid; i < units; i += AQ_WARPS * 32) {
+                const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+                *reinterpret_cast<float4*>(slot + (size_t)r * HD + d) = joined(r, d);
+            }
+            for (int r = tid; r < rows; r += AQ_WARPS * 32)
+                *reinterpret_cast<float2*>(slot + (size_t)ROWS * HD + 2 * r) = row_s[r];
+        } else {
+            for (int i = tid; i < units; i += AQ_WARPS * 32) {
+                const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+                const float l = row_s[r].y;
+                write_out(r, d, joined(r, d), l == 0.0f ? 0.0f : 1.0f / l);
+            }
+        }
+        if constexpr (MODE != AQ_SHARED) return;
+        todo -= page1 - page0;
+        if (todo <= 0) return;
+        // on to the next item
+        page0 = 0;
+        if (++item == row.items) {
+            item = 0;
+            do row = aq_row(a, ++b, ROWS); while (row.pages == 0);
+        }
+        __syncthreads();                       // everybody is done with the joined results
+    }
+    }
+}
+
+// Items that several blocks of AQ_SHARED have worked on: their results joined in the blocks' order.  Block c of a
+// row r of the grid joins matrix row r of the item that block c of the attention kernel began in, if it was the
+// second to work on it: its warps share the results out, a lane takes four dimensions.
+#define AQ_JOIN_WARPS 4
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(AQ_JOIN_WARPS * 32) attention_q8_join_kernel(AttnQ8Args a, int blocks) {
+    pdl_launch_dependents();
+    __shared__ float4 acc_s[AQ_JOIN_WARPS][HD / 4];
+    __shared__ float2 ml_s[AQ_JOIN_WARPS];
+    const int c = blockIdx.x + 1, r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    const AqFirst at_c = ((const AqFirst*)a.partial)[c];
+    if (at_c.share == 0 || at_c.page0 == 0 || at_c.page0 > at_c.share) return;
+    const AqRow row = aq_row(a, at_c.row, ROWS);
+    const int G = a.n_heads / a.n_kv, hk = at_c.item % a.n_kv, at = at_c.item / a.n_kv * ROWS + r;
+    if (at >= row.count * G) return;
+    const int c0 = c - 1, c1 = c + (row.pages - at_c.page0 - 1) / at_c.share;
+    const float* slots = a.partial + aq_table_floats(blocks);
+    auto slot = [&](int c) { return slots + (2 * (size_t)c + (c == c0 ? 1 : 0)) * aq_slot_floats(ROWS, HD); };
+    const bool mine = lane < HD / 4;
+    float m = AQ_NEG, l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int first = c0 + warp; first <= c1; first += 4 * AQ_JOIN_WARPS) {
+        float2 ml[4];
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = first + AQ_JOIN_WARPS * i;
+            ml[i] = make_float2(AQ_NEG, 0.0f);
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (c <= c1) {
+                ml[i] = *reinterpret_cast<const float2*>(slot(c) + ROWS * HD + 2 * r);
+                if (mine) x[i] = *reinterpret_cast<const float4*>(slot(c) + (size_t)r * HD + 4 * lane);
+            }
+        }
+        const float top = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+        const float m_use = top == AQ_NEG ? 0.0f : top, keep = exp2f(m - m_use);
+        m = top;
+        l *= keep;
+        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float f = exp2f(ml[i].x - m_use);
+            l = fmaf(ml[i].y, f, l);
+            acc.x = fmaf(x[i].x, f, acc.x); acc.y = fmaf(x[i].y, f, acc.y);
+            acc.z = fmaf(x[i].z, f, acc.z); acc.w = fmaf(x[i].w, f, acc.w);
         }
     }
+    if (mine) acc_s[warp][lane] = acc;
+    if (lane == 0) ml_s[warp] = make_float2(m, l);
+    __syncthreads();
+    if (threadIdx.x >= HD / 4) return;
+    float top = AQ_NEG, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < AQ_JOIN_WARPS; ++w) top = fmaxf(top, ml_s[w].x);
+    const float m_use = top == AQ_NEG ? 0.0f : top;
+    float4 out = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < AQ_JOIN_WARPS; ++w) {
+        const float f = exp2f(ml_s[w].x - m_use);
+        const float4 x = acc_s[w][threadIdx.x];
+        sum = fmaf(ml_s[w].y, f, sum);
+        out.x = fmaf(x.x, f, out.x); out.y = fmaf(x.y, f, out.y);
+        out.z = fmaf(x.z, f, out.z); out.w = fmaf(x.w, f, out.w);
+    }
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int token = at / G, head = hk * G + at - token * G;
+    const __nv_bfloat162 x = __floats2bfloat162_rn(out.x * by, out.y * by);
+    const __nv_bfloat162 y = __floats2bfloat162_rn(out.z * by, out.w * by);
+    *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(row.tok0 + token) * a.n_heads + head) * HD + 4 * threadIdx.x) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
 // ------------------------------------------------------------------------------------------
@@ -704,6 +952,11 @@ __global__ void attention_q8_merge_kernel(const float* partial, T* __restrict__ 
 // ---- host side ------------------------------------------------------------------------------
 static bool aq_on_tensor_cores(int hd, int dtype) { return dtype == MF_DTYPE_BF16 && (hd == 64 || hd == 128); }
 
+// blocks of the tensor-core kernel that an SM holds (its registers are cut for them)
+static constexpr int aq_blocks_an_sm(int hd, int rows) {
+    return hd == 128 ? (rows == 16 ? 3 : 2) : (rows <= 16 ? 4 : 3);
+}
+
 // matrix rows a block takes, from the most tokens a row brings
 static int aq_block_rows(int max_row_tokens, int group, int hd, int dtype) {
     if (!aq_on_tensor_cores(hd, dtype)) return AG_ROWS;
@@ -713,34 +966,51 @@ static int aq_block_rows(int max_row_tokens, int group, int hd, int dtype) {
     return (int)((tiles + blocks - 1) / blocks) * 8;
 }
 
-#define AQ_CLUSTER 8                           // most splits that are joined in a cluster
-// Into how many parts a row's keys are split.  `span`: the most positions the queries of one block can see,
-// from a page's border on.
-extern "C" int mf_attention_q8_plan(int n_rows, int max_row_tokens, int span, int n_heads, int n_kv, int hd, int dtype) {
-    if (n_rows <= 0 || max_row_tokens <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv != 0) return 1;
-    const int br = aq_block_rows(max_row_tokens, n_heads / n_kv, hd, dtype);
-    const long long groups = ((long long)max_row_tokens * (n_heads / n_kv) + br - 1) / br;
+#define AQ_CLUSTER 8                           // most blocks of AQ_SPLIT's clusters
+// How a call is shared out.  Tensor cores: AQ_WHOLE (splits 1), AQ_SPLIT (2, 4, 8) or AQ_SHARED (its blocks as a
+// negative number); generic kernel: the splits of a row's keys.  `span`: the most positions the queries of
+// one block can see, from a page's border on.  `floats`: the scratch it takes.
+struct AqPlan {
+    int rows, splits;
+    long long floats;
+};
+static AqPlan aq_plan(int n_tokens, int n_rows, int max_row_tokens, int span, int n_heads, int n_kv, int hd, int dtype) {
+    AqPlan p{};
+    const int group = n_heads / n_kv;
+    p.rows = aq_block_rows(max_row_tokens, group, hd, dtype);
+    const long long groups = ((long long)max_row_tokens * group + p.rows - 1) / p.rows;
     const long long items = (long long)n_rows * n_kv * groups;
-    const int pages = span <= 0 ? 1 : (span + MF_PAGE - 1) / MF_PAGE;
-    static const int forced = getenv("AQ_SPLITS") ? atoi(getenv("AQ_SPLITS")) : 0;
-    long long splits = forced ? forced : 3LL * mf_sm_count() / items;
-    if (splits > (pages + 3) / 4) splits = (pages + 3) / 4;      // 256 keys a split at least
-    if (splits > AQ_MAX_SPLITS) splits = AQ_MAX_SPLITS;
-    if (splits < 1) splits = 1;
-    if (aq_on_tensor_cores(hd, dtype) && splits <= 2 * AQ_CLUSTER) {
-        int s = 1;
-        while (2 * s <= splits && 2 * s <= AQ_CLUSTER) s *= 2;
-        splits = s;
+    const int pages = span <= 0 ? 1 : (span + MF_PAGE - 1) / MF_PAGE, sms = mf_sm_count();
+    if (!aq_on_tensor_cores(hd, dtype)) {
+        long long splits = 3LL * sms / items;
+        if (splits > (pages + 3) / 4) splits = (pages + 3) / 4;          // 256 keys a split at least
+        if (splits > AQ_MAX_SPLITS) splits = AQ_MAX_SPLITS;
+        p.splits = splits < 1 ? 1 : (int)splits;
+        p.floats = p.splits > 1 ? (long long)n_tokens * n_heads * p.splits * (hd + 2) : 0;
+        return p;
     }
-    return (int)splits;
+    const int held = sms * aq_blocks_an_sm(hd, p.rows);
+    int cluster = 1;
+    while (2 * cluster <= AQ_CLUSTER && 2 * cluster * items <= held && 2 * cluster <= (pages + 3) / 4) cluster *= 2;
+    // Clusters where they fill half of the GPU at least, or where a block has 12 pages at most; a block an item
+    // where that is little.  us, whole / clusters / shared: 8 sequences at 2,000 positions (28 heads, 4 of
+    // keys) - / 10.3 / 14.4, at 32,000 - / 48.0 / 53.0; 1 at 32,000 - / 39 / 20; 64 of 0 to 4,095 (14 and 2 heads of 64) -
+    // / 16.4 / 26.6; 64 of 2,047 to 8,100 80 / - / 65; 128 of 500 23.1 / - / 27.4, of 2,000 64 / - / 55.
+    if ((pages <= 12 || cluster > 1) && (pages <= 12 * cluster || 2LL * cluster * items >= held)) {
+        p.splits = cluster;
+        return p;
+    }
+    p.splits = -held;
+    p.floats = (long long)aq_table_floats(held) + 2LL * held * (long long)aq_slot_floats(p.rows, hd);
+    return p;
 }
 
 #define AQ_MAX_DEVICES 64
-template <int HD, int FMT, int NT, bool CLUSTER, int STAGES, int MINB>
-static int launch_mma_as(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
-    constexpr int ring = AQ_WARPS * STAGES * AqTile<HD>::STAGE, join = AQ_WARPS * 8 * NT * (HD + 4) * 4;
+template <int HD, int FMT, int NT, int KT, int MODE, int STAGES, int MINB>
+static int launch_mma_as(const AttnQ8Args& a, int items, int blocks, cudaStream_t stream) {
+    constexpr int ring = AQ_WARPS * STAGES * KT * AqTile<HD>::STAGE, join = AQ_WARPS * 8 * NT * (HD + 4) * 4;
     constexpr int smem = ring > join ? ring : join;
-    auto kernel = attention_q8_mma_kernel<HD, FMT, NT, CLUSTER, STAGES, MINB>;
+    auto kernel = attention_q8_mma_kernel<HD, FMT, NT, KT, MODE, STAGES, MINB>;
     static bool opened[AQ_MAX_DEVICES] = {};
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
@@ -748,8 +1018,12 @@ static int launch_mma_as(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
         if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return (int)e;
         if (dev >= 0 && dev < AQ_MAX_DEVICES) opened[dev] = true;
     }
-    if (!CLUSTER) {
+    const dim3 grid = MODE == AQ_SHARED ? dim3(blocks) : dim3(a.n_splits, items, a.n_rows);
+    if (MODE != AQ_SPLIT) {
         mf_launch(kernel, grid, dim3(AQ_WARPS * 32), smem, stream, a);
+        if (int e = MF_LAUNCH_CHECK()) return e;
+        if (MODE == AQ_SHARED && blocks > 1)
+            mf_launch(attention_q8_join_kernel<HD, 8 * NT>, dim3(blocks - 1, 8 * NT), dim3(AQ_JOIN_WARPS * 32), 0, stream, a, blocks);
         return MF_LAUNCH_CHECK();
     }
     cudaLaunchConfig_t cfg = {};
@@ -767,11 +1041,12 @@ static int launch_mma_as(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
     cudaLaunchKernelEx(&cfg, kernel, a);
     return MF_LAUNCH_CHECK();
 }
-template <int HD, int FMT, int NT, int STAGES, int MINB>
-static int launch_mma(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
-    return a.n_splits > 1 && a.n_splits <= AQ_CLUSTER
-               ? launch_mma_as<HD, FMT, NT, true, STAGES, MINB>(a, grid, stream)
-               : launch_mma_as<HD, FMT, NT, false, STAGES, MINB>(a, grid, stream);
+template <int HD, int FMT, int NT, int KT, int STAGES>
+static int launch_mma(const AttnQ8Args& a, int items, int splits, cudaStream_t stream) {
+    constexpr int minb = aq_blocks_an_sm(HD, 8 * NT);
+    return splits < 0    ? launch_mma_as<HD, FMT, NT, KT, AQ_SHARED, STAGES, minb>(a, items, -splits, stream)
+           : splits == 1 ? launch_mma_as<HD, FMT, NT, KT, AQ_WHOLE, STAGES, minb>(a, items, 0, stream)
+                         : launch_mma_as<HD, FMT, NT, KT, AQ_SPLIT, STAGES, minb>(a, items, 0, stream);
 }
 template <typename T, int FMT> static int launch_generic(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
     const int smem = (AG_KEYS * (2 * a.hd + 1) + AG_ROWS * a.hd + 2 * AG_KEYS + AG_ROWS * AG_KEYS) * 4;
@@ -789,27 +1064,32 @@ template <typename T, int FMT> static int launch_generic(const AttnQ8Args& a, di
     return MF_LAUNCH_CHECK();
 }
 
-// Whether so many splits are joined by a second kernel, from partial results.
-extern "C" int mf_attention_q8_merges(int n_splits, int hd, int dtype) {
-    return n_splits > (aq_on_tensor_cores(hd, dtype) ? AQ_CLUSTER : 1);
+// The scratch of a call in floats; `kernels`: how many it launches.
+extern "C" long long mf_attention_q8_plan(int n_tokens, int n_rows, int max_row_tokens, int span, int n_heads, int n_kv,
+                                          int hd, int dtype, int* kernels) {
+    *kernels = 1;
+    if (n_rows <= 0 || max_row_tokens <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv != 0) return 0;
+    const AqPlan p = aq_plan(n_tokens, n_rows, max_row_tokens, span, n_heads, n_kv, hd, dtype);
+    *kernels = p.floats > 0 ? 2 : 1;
+    return p.floats;
 }
 
-// `n_splits`: any number from 1 on (mf_attention_q8_plan gives a good one); `partial` holds
-// tokens * n_heads * n_splits * (hd + 2) floats where mf_attention_q8_merges says so.
+// `partial` holds what mf_attention_q8_plan says for the same sizes, 16-byte aligned.
 extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v_codes, const float* k_scales,
                                const float* v_scales, const int* cu_seqlens, const int* seq_end, const int* page_table,
                                int table_stride, int ring, int n_pages, void* out, float* partial, int n_tokens,
-                               int n_rows, int max_row_tokens, int n_heads, int n_kv, int hd, int window, int n_splits,
+                               int n_rows, int max_row_tokens, int span, int n_heads, int n_kv, int hd, int window,
                                float scale, int dtype, int fmt, unsigned* status, cudaStream_t stream) {
     if (n_tokens <= 0 || n_rows <= 0 || max_row_tokens <= 0) return 0;
     if (hd % 16 != 0 || hd < 16 || hd > 256 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv != 0) return MF_ERR_UNSUPPORTED;
     if ((dtype != MF_DTYPE_F32 && dtype != MF_DTYPE_BF16) || (fmt != MF_Q8_E4M3 && fmt != MF_Q8_INT8))
         return MF_ERR_UNSUPPORTED;
-    if (table_stride <= 0 || n_pages <= 0 || ring < 0 || ring % MF_PAGE != 0 || window < 0 || n_splits < 1 ||
-        (partial == nullptr && mf_attention_q8_merges(n_splits, hd, dtype)) || status == nullptr)
+    if (table_stride <= 0 || n_pages <= 0 || ring < 0 || ring % MF_PAGE != 0 || window < 0 || status == nullptr)
         return MF_ERR_ARGUMENT;
+    const AqPlan plan = aq_plan(n_tokens, n_rows, max_row_tokens, span, n_heads, n_kv, hd, dtype);
+    if (plan.floats > 0 && (partial == nullptr || ((uintptr_t)partial & 15))) return MF_ERR_ARGUMENT;
     if (ring > 0 && (window <= 0 || max_row_tokens > ring - window + 1)) return MF_ERR_ARGUMENT;
-    if (n_rows > 65535 || n_splits > AQ_MAX_SPLITS) return MF_ERR_UNSUPPORTED;
+    if (n_rows > 65535) return MF_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales |
          (uintptr_t)out) & 15)
         return MF_ERR_UNSUPPORTED;
@@ -817,22 +1097,21 @@ extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v
     a.q = q; a.k_codes = (const uint8_t*)k_codes; a.v_codes = (const uint8_t*)v_codes; a.k_scales = k_scales;
     a.v_scales = v_scales; a.cu_seqlens = cu_seqlens; a.seq_end = seq_end; a.page_table = page_table;
     a.table_stride = table_stride; a.ring = ring; a.n_pages = n_pages; a.out = out; a.partial = partial;
-    a.n_tokens = n_tokens; a.n_heads = n_heads; a.n_kv = n_kv; a.hd = hd; a.window = window;
-    a.n_splits = n_splits; a.scale = scale; a.status = status;
-    const int G = n_heads / n_kv, br = aq_block_rows(max_row_tokens, G, hd, dtype);
-    const long long groups = ((long long)max_row_tokens * G + br - 1) / br;
-    if (groups * n_kv > 65535) return MF_ERR_UNSUPPORTED;
+    a.n_tokens = n_tokens; a.n_rows = n_rows; a.n_heads = n_heads; a.n_kv = n_kv; a.hd = hd; a.window = window;
+    a.n_splits = plan.splits < 0 ? 1 : plan.splits; a.scale = scale; a.status = status;
+    const long long groups = ((long long)max_row_tokens * (n_heads / n_kv) + plan.rows - 1) / plan.rows;
+    if (groups * n_kv > 32767) return MF_ERR_UNSUPPORTED;
     a.q_groups = (int)groups;
-    const dim3 grid(n_splits, (unsigned)(groups * n_kv), n_rows);
+    const int items = (int)(groups * n_kv), n_splits = a.n_splits;
+    const dim3 grid(n_splits, items, n_rows);
     int e;
     if (aq_on_tensor_cores(hd, dtype)) {
-#define AQ_GO(HD, NT, STAGES, MINB)                                                      \
-    (fmt == MF_Q8_E4M3 ? launch_mma<HD, MF_Q8_E4M3, NT, STAGES, MINB>(a, grid, stream)   \
-                       : launch_mma<HD, MF_Q8_INT8, NT, STAGES, MINB>(a, grid, stream))
-        if (hd == 128)
-            e = br == 8 ? AQ_GO(128, 1, 4, 3) : br == 16 ? AQ_GO(128, 2, 4, 3) : br == 24 ? AQ_GO(128, 3, 4, 2) : AQ_GO(128, 4, 4, 2);
-        else
-            e = br == 8 ? AQ_GO(64, 1, 6, 4) : br == 16 ? AQ_GO(64, 2, 6, 4) : br == 24 ? AQ_GO(64, 3, 6, 4) : AQ_GO(64, 4, 6, 3);
+#define AQ_GO(HD, NT, KT, STAGES)                                                                 \
+    (fmt == MF_Q8_E4M3 ? launch_mma<HD, MF_Q8_E4M3, NT, KT, STAGES>(a, items, plan.splits, stream) \
+                       : launch_mma<HD, MF_Q8_INT8, NT, KT, STAGES>(a, items, plan.splits, stream))
+        const int nt = plan.rows / 8;
+        if (hd == 128) return nt == 1 ? AQ_GO(128, 1, 2, 3) : nt == 2 ? AQ_GO(128, 2, 1, 4) : nt == 3 ? AQ_GO(128, 3, 1, 4) : AQ_GO(128, 4, 1, 4);
+        return nt == 1 ? AQ_GO(64, 1, 2, 3) : nt == 2 ? AQ_GO(64, 2, 1, 6) : nt == 3 ? AQ_GO(64, 3, 1, 6) : AQ_GO(64, 4, 1, 6);
 #undef AQ_GO
     } else if (dtype == MF_DTYPE_F32) {
         e = fmt == MF_Q8_E4M3 ? launch_generic<float, MF_Q8_E4M3>(a, grid, stream)
@@ -841,7 +1120,7 @@ extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v
         e = fmt == MF_Q8_E4M3 ? launch_generic<__nv_bfloat16, MF_Q8_E4M3>(a, grid, stream)
                               : launch_generic<__nv_bfloat16, MF_Q8_INT8>(a, grid, stream);
     }
-    if (e || !mf_attention_q8_merges(n_splits, hd, dtype)) return e;
+    if (e || n_splits == 1) return e;
     const int threads = hd >= 128 ? 128 : hd >= 64 ? 64 : 32;
     if ((long long)n_tokens * n_heads > 0x7fffffffLL) return MF_ERR_UNSUPPORTED;
     if (dtype == MF_DTYPE_F32)

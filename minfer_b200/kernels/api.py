@@ -395,13 +395,13 @@ def _sig_moe(lib: ctypes.CDLL) -> None:
 def _sig_cache_q8(lib: ctypes.CDLL) -> None:
     lib.mf_rope_kvstore_q8.argtypes = ([c_void_p, c_int] + [c_void_p] * 13 + [c_int] * 11 +
                                        [c_void_p, c_void_p])
-    lib.mf_read_pages_q8.argtypes = ([c_void_p] * 5 + [c_int] * 3 + [c_void_p] * 3 + [c_int] * 6 +
+    lib.mf_read_pages_q8.argtypes = ([c_void_p] * 5 + [c_int] * 4 + [c_void_p] * 3 + [c_int] * 7 +
                                      [c_void_p, c_void_p])
 
 
 def _sig_attention_q8(lib: ctypes.CDLL) -> None:
-    lib.mf_attention_q8_plan.argtypes = [c_int] * 7
-    lib.mf_attention_q8_merges.argtypes = [c_int] * 3
+    lib.mf_attention_q8_plan.argtypes = [c_int] * 8 + [c_void_p]
+    lib.mf_attention_q8_plan.restype = c_longlong
     lib.mf_attention_q8.argtypes = ([c_void_p] * 8 + [c_int] * 3 + [c_void_p, c_void_p] + [c_int] * 8 +
                                     [c_float, c_int, c_int, c_void_p, c_void_p])
 
@@ -1149,6 +1149,16 @@ def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]
             raise KernelError(f"{what}: tensors on {first.device} and {t.device}")
 
 
+_sms_of: Dict[int, int] = {}
+
+
+def sm_count(device: torch.device) -> int:
+    index = device.index
+    if index not in _sms_of:
+        _sms_of[index] = torch.cuda.get_device_properties(index).multi_processor_count
+    return _sms_of[index]
+
+
 def _table(page_table: torch.Tensor, table_stride: int, rows: int, what: str) -> None:
     if table_stride < 1 or page_table.numel() < rows * table_stride:
         raise KernelError(f"{what}: the page table is smaller than {rows} rows of {table_stride} pages")
@@ -1221,30 +1231,62 @@ def read_pages_q8(pages: Q8Pages, page_table: torch.Tensor, table_stride: int, r
     if k_out.dtype != v_out.dtype or k_out.numel() != want or v_out.numel() != want:
         raise KernelError(f"{what}: the outputs must be [rows * table_stride, {n_kv}, {PAGE}, {head_dim}] of one type")
     _same_device(what, *pages, page_table, seq_end, k_out, v_out, status)
+    _read_pages_q8(pages, fmt, page_table, table_stride, table_stride, ring, seq_end, k_out, v_out, status, fill, False)
+
+
+def _read_pages_q8(pages: Q8Pages, fmt: int, page_table: torch.Tensor, table_stride: int, out_stride: int, ring: int,
+                   seq_end: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, status: torch.Tensor, fill: bool,
+                   for_attention: bool) -> None:
+    """``out_stride`` pages a row in the output (behind the table's: zeros).  ``for_attention``: a position whose
+    key or value is NaN becomes a key of NaN with a value of zeros."""
     _check(_lib("cache_q8").mf_read_pages_q8(
         _ptr(pages.k, "keys"), _ptr(pages.v, "values"), _ptr(pages.k_scale, "key scales"),
-        _ptr(pages.v_scale, "value scales"), _i32(page_table, "page_table"), int(table_stride), int(ring),
-        pages.k.shape[0], _i32(seq_end, "seq_end"), _ptr(k_out, "k_out"), _ptr(v_out, "v_out"), rows, n_kv, head_dim,
-        dtype_code(k_out.dtype), fmt, 1 if fill else 0, _i32(status, "status"), _stream()), what)
+        _ptr(pages.v_scale, "value scales"), _i32(page_table, "page_table"), int(table_stride),
+        int(out_stride), int(ring), pages.k.shape[0], _i32(seq_end, "seq_end"), _ptr(k_out, "k_out"),
+        _ptr(v_out, "v_out"), seq_end.numel(), pages.k.shape[1], pages.k.shape[3], dtype_code(k_out.dtype), fmt,
+        1 if fill else 0, 1 if for_attention else 0, _i32(status, "status"), _stream()), "read_pages_q8")
 
 
 _Q8_PLANS: Dict[tuple, tuple] = {}
 
 
-def attention_q8_plan(n_rows: int, max_row_tokens: int, span: int, n_heads: int, n_kv: int, head_dim: int,
-                      dtype: torch.dtype) -> tuple[int, bool]:
-    """(parts that a row's keys are split into, whether a second kernel joins them) of attention over 8-bit
-    pages; ``span``: the most positions that the queries of a row see."""
-    key = (torch.cuda.current_device(), n_rows, max_row_tokens, span, n_heads, n_kv, head_dim, dtype)
+def attention_q8_plan(n_tokens: int, n_rows: int, max_row_tokens: int, span: int, n_heads: int, n_kv: int,
+                      head_dim: int, dtype: torch.dtype) -> tuple[int, int]:
+    """(floats of scratch, kernels) that attention over 8-bit pages takes; ``span``: the most positions that
+    the queries of a row see."""
+    key = (torch.cuda.current_device(), n_tokens, n_rows, max_row_tokens, span, n_heads, n_kv, head_dim, dtype)
     got = _Q8_PLANS.get(key)
     if got is None:
-        lib, code = _lib("attention_q8"), dtype_code(dtype)
-        splits = lib.mf_attention_q8_plan(n_rows, max_row_tokens, span, n_heads, n_kv, head_dim, code)
-        got = (splits, bool(lib.mf_attention_q8_merges(splits, head_dim, code)))
+        kernels = c_int(0)
+        floats = _lib("attention_q8").mf_attention_q8_plan(n_tokens, n_rows, max_row_tokens, span, n_heads, n_kv,
+                                                           head_dim, dtype_code(dtype), ctypes.addressof(kernels))
+        got = (floats, kernels.value)
         if len(_Q8_PLANS) > 4096:
             _Q8_PLANS.clear()
         _Q8_PLANS[key] = got
     return got
+
+
+Q8_PORTION_BYTES = 2 << 30      # of pages read back at a time
+
+
+def q8_reads_back(tokens: int, rows: int, max_row_tokens: int, span: int, n_heads: int, n_kv: int, head_dim: int,
+                  sms: int) -> bool:
+    """Whether attention over 8-bit pages reads them back into bfloat16 and runs the tcgen05 kernel of portions
+    (query tiles of 256 tokens of one head) instead of multiplying codes on mma.sync (all heads of a group
+    and all tokens of a row share the keys).  Both times are estimated from what they were measured at, for
+    rows of ``span`` positions: the tcgen05 kernel walks a row's keys at 14 ns each (12 at head size 64) in as
+    many rounds as its blocks need of the SMs, behind 3 bytes a code at 5 TB/s; the other does 225 TFLOP/s
+    (165).  Measured on both sides, us, codes against read back, 28 heads / 4 of 128 over 4,000 positions: 1 row
+    of 128 tokens 54 / 70, of 256 92 / 77; 8 rows of 32 90 / 142, of 128 290 / 152; 14 / 2 of 64: 1 row of 256
+    41 / 70, 8 rows of 64 68 / 59, 32 rows of 32 109 / 215, of 64 187 / 217, of 128 345 / 226."""
+    if max_row_tokens < 32:
+        return False
+    wide = head_dim == 128
+    rounds = -(-n_heads * rows * -(-max_row_tokens // 256) // sms)
+    back = rounds * span * (14e-9 if wide else 12e-9) + rows * span * n_kv * head_dim * 6 / 5e12 + 8e-6
+    codes = 4.0 * tokens * span * n_heads * head_dim / (225e12 if wide else 165e12) + 4e-6
+    return back < codes
 
 
 def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor, seq_end: torch.Tensor,
@@ -1256,7 +1298,9 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
     and the pages hold every position up to there, the step's own included.  A token sees the positions up
     to its own (the last ``window`` of them where that is not 0) and reads zeros if there is none.
     ``max_row_tokens``: the most tokens a row brings; ``max_end``: a bound of ``seq_end`` (it sizes the splits).
-    A page that a token would see and its row has not counts as not seen and sets status bit 2."""
+    A page that a token would see and its row has not sets status bit 2; what such a row reads is undefined, but
+    nothing outside the pages is touched and other rows are not.  Long portions are read back into bfloat16 first
+    (``q8_reads_back``), in scratch of at most ``Q8_PORTION_BYTES`` or one row's pages."""
     what = "attention_paged_q8"
     rows, tokens = seq_end.numel(), q.shape[0]
     if n_kv < 1 or n_heads < 1 or n_heads % n_kv != 0:
@@ -1278,17 +1322,31 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
     span = int(max_end)
     if window > 0:                    # from a page's border on
         span = min(span, window + int(max_row_tokens) + PAGE - 1)
-    n_splits, merges = attention_q8_plan(rows, int(max_row_tokens), span, n_heads, n_kv, head_dim, q.dtype)
-    partial = None
-    if merges:
-        partial = torch.empty(tokens * n_heads * n_splits * (head_dim + 2), dtype=torch.float32, device=q.device)
+    if q.dtype == torch.bfloat16 and head_dim in (64, 128) and q8_reads_back(
+            tokens, rows, int(max_row_tokens), span, n_heads, n_kv, head_dim, sm_count(q.device)):
+        # pages of the rows read back, as many rows at a time as the scratch takes; a tile of the kernel is
+        # two pages, so a row has an even number of them (the last one zeros where there is none)
+        wide = table_stride + (table_stride & 1)
+        some = max(1, min(rows, Q8_PORTION_BYTES // (wide * n_kv * PAGE * head_dim * 4)))
+        k = torch.empty((some * wide, n_kv, PAGE, head_dim), dtype=torch.bfloat16, device=q.device)
+        v = torch.empty_like(k)
+        places = torch.arange(some * wide, dtype=torch.int32, device=q.device)
+        for first in range(0, rows, some):
+            last = min(rows, first + some)
+            ends = seq_end[first:last]
+            _read_pages_q8(pages, fmt, page_table.view(-1)[first * table_stride:], table_stride, wide, ring, ends, k, v,
+                           status, True, True)
+            attention_prefill_tc_paged(q, k, v, cu_seqlens[first:last + 1], ends, places, wide, ring, out, last - first,
+                                       int(max_row_tokens), n_heads, n_kv, head_dim, int(window), float(scale), status)
+        return
+    floats, kernels = attention_q8_plan(tokens, rows, int(max_row_tokens), span, n_heads, n_kv, head_dim, q.dtype)
+    partial = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     _check(_lib("attention_q8").mf_attention_q8(
         _ptr(q, "q"), _ptr(pages.k, "keys"), _ptr(pages.v, "values"), _ptr(pages.k_scale, "key scales"),
         _ptr(pages.v_scale, "value scales"), _i32(cu_seqlens, "cu_seqlens"), _i32(seq_end, "seq_end"),
         _i32(page_table, "page_table"), int(table_stride), int(ring), pages.k.shape[0], _ptr(out, "out"),
-        _f32(partial, "partial"), tokens, rows, int(max_row_tokens), n_heads, n_kv, head_dim, int(window),
-        n_splits, float(scale), dtype_code(q.dtype), fmt, _i32(status, "status"), _stream()), what,
-        2 if merges else 1)
+        _f32(partial, "partial"), tokens, rows, int(max_row_tokens), span, n_heads, n_kv, head_dim,
+        int(window), float(scale), dtype_code(q.dtype), fmt, _i32(status, "status"), _stream()), what, kernels)
 
 
 # ---------------------------------------------------------------------------------------

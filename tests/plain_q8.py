@@ -99,6 +99,15 @@ def attention_tolerance(want, mass, top, size, keys, dtype, dim, fmt):
     return mass * rel[..., None] + small[..., None] + want.abs() * 2.0 ** -8 + 1e-37
 
 
+def read_back_tolerance(want, mass, top, size, keys):
+    """The same where keys and values are read back into bfloat16 first: each is rounded (2^-8, and its product
+    with the scale 2^-24 before), so a score is off by 2^-8 of the sum of its products' magnitudes and a
+    probability relatively by twice that (its own and the sum's); probabilities are rounded to bfloat16 for the
+    second product (2^-8), values are (2^-8), and so is the output (2^-8)."""
+    rel = 2 * (2.0 ** -8 + 2.0 ** -14) * size + 2 * 2.0 ** -8 + 2.0 ** -12
+    return mass * rel[..., None] + want.abs() * 2.0 ** -8 + 1e-37
+
+
 def softmax(row, temperature):
     d = row.astype(np.float64)
     if np.isnan(d).any() or np.isposinf(d).any() or not (d > -np.inf).any():

@@ -217,7 +217,7 @@ def test_tokens_of_other_rows_are_left_alone_where_keys_are_split(dtype, dim):
     table, n_pages = make_table(ends, 0, rng)
     pages = make_pages(table, n_pages, ends, 0, kv, dim, fmt, gen)
     q = torch.randn(8, heads, dim, generator=gen).to(dtype).to(DEV)
-    assert K.attention_q8_plan(2, 2, 2000, heads, kv, dim, dtype)[0] > 1
+    assert dtype == torch.bfloat16 or K.attention_q8_plan(8, 2, 2, 2000, heads, kv, dim, dtype)[0] > 0
     out = torch.full_like(q, 7.0)
     K.attention_paged_q8(q, pages, ints(cu), ints(ends), ints(table), len(table[0]), 0, out, 2, 2000, heads, kv, dim, 0,
                          0.2, status_word())
@@ -305,6 +305,45 @@ def test_captured_twice_and_on_another_stream():
         K.attention_paged_q8(qs[0], pages, cu_d, end_d, table_d, len(table[0]), 0, out, 1, 1500, heads, kv, dim, 0, 0.1, st)
     side.synchronize()
     assert torch.equal(out, eager[0])
+
+
+@FORMATS
+@pytest.mark.parametrize("heads,kv,dim", [(6, 2, 128), (14, 2, 64), (3, 3, 64)])
+@pytest.mark.parametrize("rows,window", [([(40, 0)], 0), ([(100, 29), (1, 300), (33, 64), (129, 0)], 0),
+                                         ([(70, 500), (64, 0), (3, 127)], 90)])
+@pytest.mark.parametrize("at_a_time", [None, 2])
+def test_portions_that_are_read_back(rows, window, heads, kv, dim, fmt, at_a_time, monkeypatch):
+    """The other way to attend, which long portions take: the same result, NaN with those who see it only
+    (a value of NaN in a later token, in another row, in a place no row sees), in one go and some rows at a
+    time."""
+    monkeypatch.setattr(K, "q8_reads_back", lambda *a: True)
+    gen, rng = torch.Generator().manual_seed(41), np.random.RandomState(6)
+    new, past = zip(*rows)
+    ends = [n + p for n, p in zip(new, past)]
+    cu = [0] + np.cumsum(new).tolist()
+    ring = -(-(window + max(new) - 1) // PAGE) * PAGE if window else 0
+    table, n_pages = make_table(ends, ring, rng)
+    if at_a_time:
+        monkeypatch.setattr(K, "Q8_PORTION_BYTES", at_a_time * (len(table[0]) + 1) * kv * PAGE * dim * 4)
+    pages = make_pages(table, n_pages, ends, ring, kv, dim, fmt, gen)
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(torch.bfloat16).to(DEV)
+    got = run_attention(q, pages, cu, ends, table, ring, heads, kv, dim, window, dim ** -0.5)
+    want, *sizes = plain.attention(q, pages, cu, ends, table, ring, heads, kv, window, dim ** -0.5)
+    tol = plain.read_back_tolerance(want, *sizes)
+    assert ((got.double().cpu() - want).abs() <= tol).all()
+    # a value of NaN at the first row's last position but one: its last two tokens see it
+    pos = ends[0] - 2
+    place = pos % ring if ring else pos
+    page = table[0][place // PAGE]
+    pages.v_scale[page, 0, place % PAGE] = float("nan")
+    pages.k_scale[page, kv - 1, place % PAGE] = float("nan")
+    bad = run_attention(q, pages, cu, ends, table, ring, heads, kv, dim, window, dim ** -0.5)
+    group = heads // kv
+    sees = torch.zeros(got.shape[:2], dtype=torch.bool)
+    sees[new[0] - 2:new[0], :group] = True
+    sees[new[0] - 2:new[0], (kv - 1) * group:] = True
+    assert torch.isnan(bad[sees.to(DEV)]).all()
+    assert torch.equal(bad[~sees.to(DEV)], got[~sees.to(DEV)])
 
 
 # ---- written and read back ------------------------------------------------------------------------
