@@ -3,7 +3,6 @@ import pytest
 import torch
 
 from minfer_b200.cache.paged import PAGE, Cache, CacheError, GroupKey, cache_dtype_of
-from minfer_b200.cli import CliError, parse_args
 
 
 def make(dtype=torch.int8, max_tokens=1024, max_seqs=4, step_tokens=1):
@@ -44,6 +43,7 @@ def test_values_of_another_shape_are_refused(key):
 
 
 def test_names_of_the_types():
+    from minfer_b200.cli import CliError, parse_args      # (here: what is imported first keeps its stdout)
     assert cache_dtype_of(None) is None
     assert cache_dtype_of("e4m3") is torch.float8_e4m3fn is cache_dtype_of(torch.float8_e4m3fn)
     assert cache_dtype_of("int8") is torch.int8
