@@ -18,9 +18,10 @@
 //
 // Two launches.  The first reads every row once: the maximum and sum of a piece of 8,192 logits, which stay
 // in registers between the two (bound by bytes).  The second joins the pieces, decides, and
-// passes over the one row that the token comes from: a cluster of eight blocks a sequence, every warp a
-// contiguous stretch of the vocabulary, whose sums all blocks see; the one warp whose stretch holds the
-// answer goes through it again.
+// passes over the one row that the token comes from: a cluster of up to eight blocks a sequence, every warp a
+// contiguous stretch of the vocabulary, whose sums all blocks see; the block whose stretch holds the answer has
+// kept that stretch's sums in steps of 128 tokens, and goes through one step again (through the whole
+// stretch, a step after the other: 25 us more).
 //
 // The token has to be the definition's: a running sum over 150,000 tokens has a border within 7e-6 of any
 // number, and within 1e-8 of one number in 300.  So everything that a draw compares is double, the
@@ -33,8 +34,10 @@
 #define DR_THREADS 256
 #define DR_EACH 32                                   // logits a thread of the first launch holds
 #define DR_PIECE (DR_THREADS * DR_EACH)
-#define DR_CLUSTER 8
+#define DR_CLUSTER 8                                 // most blocks a sequence
 #define DR_WARPS 16
+#define DR_STEPS 64                                  // most steps of a stretch
+#define DR_KEPT 32                                   // places whose maximum and sum a block keeps
 
 struct DraftArgs {
     const float* logits;                             // [n_drafts + n_seqs] rows
@@ -174,20 +177,32 @@ __global__ void __launch_bounds__(DR_THREADS) draft_pieces_kernel(DraftArgs a) {
     }
 }
 
-// a row's maximum and sum from its pieces (every lane of the warp gets them)
-__device__ __forceinline__ void join_pieces(const DraftArgs& a, int row, float* top, double* sum) {
+// a row's maximum and sum from its pieces (every lane of the warp gets them; NaN: no distribution)
+struct RowSum {
+    double sum;
+    float top;
+};
+__device__ __forceinline__ RowSum join_pieces(const DraftArgs& a, int row, const double* table) {
     const double2* p = a.pieces + (size_t)row * a.n_pieces;
     const int lane = threadIdx.x & 31;
-    float m = -INFINITY;
-    for (int i = lane; i < a.n_pieces; i += 32) m = fmaxf(m, (float)p[i].x);
-    m = warp_max(m);
+    const double steps = draft_steps(a);
+    RowSum r;
+    r.top = -INFINITY;
     double s = 0.0;
-    for (int i = lane; i < a.n_pieces; i += 32) {
-        const double d = p[i].x == (double)-INFINITY ? 0.0 : (double)((float)p[i].x - m) * ((double)a.inv_hi + (double)a.inv_lo);
-        s += p[i].y * exp(d);
+    // (32 pieces are 262,144 tokens: more only beyond that)
+    for (int i0 = 0; i0 < a.n_pieces; i0 += 32) {
+        const double2 v = i0 + lane < a.n_pieces ? p[i0 + lane] : make_double2((double)-INFINITY, 0.0);
+        const float mine = (float)v.x, top = fmaxf(r.top, warp_max(mine));
+        // a piece of nothing but -infinity has a sum of 0, or NaN if that is among it
+        const double off = -(double)(top == -INFINITY ? 0.0f : top) * steps;
+        const double part = v.y * (mine == -INFINITY ? 1.0 : draft_exp(mine, steps, off, table));
+        if (i0 > 0) s *= r.top == -INFINITY ? 1.0 : draft_exp(r.top, steps, off, table);
+        s += part;
+        r.top = top;
     }
-    *top = m;
-    *sum = m > -INFINITY ? warp_sum_d(s) : (double)NAN;
+    s = warp_sum_d(s);
+    r.sum = r.top > -INFINITY ? s : (double)NAN;
+    return r;
 }
 
 // Of the warp's 128 weights (four neighbours a lane): the first one whose running sum, on top of `run`, lies
@@ -238,18 +253,19 @@ __device__ __forceinline__ double sum_of_stretches(const double* sums) {
 static_assert(DR_CLUSTER * DR_WARPS == 128, "a lane takes four stretches");
 
 template <bool VEC>
-__global__ void __launch_bounds__(DR_WARPS * 32) draft_resolve_kernel(DraftArgs a) {
+__global__ void __launch_bounds__(DR_WARPS * 32) draft_resolve_kernel(DraftArgs a, int blocks) {
     namespace cg = cooperative_groups;
     __shared__ double table_s[DR_TABLE];
+    __shared__ double sums_s[2][DR_CLUSTER * DR_WARPS];      // the stretches' sums, of every warp of the cluster
+    __shared__ double steps_s[DR_WARPS][DR_STEPS];           // this block's stretches, step by step
+    __shared__ RowSum rows_s[DR_KEPT][2];                    // of the first places: target, draft
+    __shared__ int stop_s;
     draft_table(table_s);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = blockIdx.x % blocks, b = blockIdx.x / blocks;
+    if (tid < 2 * DR_CLUSTER * DR_WARPS) sums_s[0][tid] = 0.0;
     pdl_prologue();
     cg::cluster_group cluster = cg::this_cluster();
-    __shared__ double sums_s[2][DR_CLUSTER * DR_WARPS];      // the stretches' sums, of every warp of the cluster
-    __shared__ int stop_s;
-    __shared__ float top_s[2];
-    __shared__ double all_s[2];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = blockIdx.x % DR_CLUSTER, b = blockIdx.x / DR_CLUSTER;
     const int d0 = a.cu[b], n = a.cu[b + 1] - d0;
     const bool fits = d0 >= 0 && n >= 0 && d0 + n <= a.n_drafts;       // (uniform over the cluster)
     const int row0 = d0 + b, n_target = a.n_drafts + a.n_seqs;
@@ -261,131 +277,134 @@ __global__ void __launch_bounds__(DR_WARPS * 32) draft_resolve_kernel(DraftArgs 
     __syncthreads();
     if (a.greedy) {
         if (rank != 0) return;                               // (no block of this cluster waits for another)
-        for (int j = warp; j <= n; j += DR_WARPS) {
+        // the first maximum of place j, -1 if there is none
+        auto first_of = [&](int j) {
             const double2* p = a.pieces + (size_t)(row0 + j) * a.n_pieces;
             unsigned long long best = 0;
             bool bad = false;
             for (int i = lane; i < a.n_pieces; i += 32) {
-                best = max(best, (unsigned long long)__double_as_longlong(p[i].x));
-                bad |= p[i].y != 0.0;
+                const double2 v = p[i];
+                best = max(best, (unsigned long long)__double_as_longlong(v.x));
+                bad |= v.y != 0.0;
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
             bad = __any_sync(0xffffffffu, bad) || best == 0;
-            const int first = bad ? -1 : 0x7fffffff - (int)(best & 0xffffffffu);
-            if (lane == 0 && j < n && first != a.drafts[d0 + j]) atomicMin(&stop_s, j);
+            return bad ? -1 : 0x7fffffff - (int)(best & 0xffffffffu);
+        };
+        for (int j = warp; j < n; j += DR_WARPS) {
+            const int first = first_of(j);
+            if (lane == 0 && (first < 0 || first != a.drafts[d0 + j])) atomicMin(&stop_s, j);
         }
         __syncthreads();
         if (warp == 0) {
-            const double2* p = a.pieces + (size_t)(row0 + stop_s) * a.n_pieces;
-            unsigned long long best = 0;
-            bool bad = false;
-            for (int i = lane; i < a.n_pieces; i += 32) {
-                best = max(best, (unsigned long long)__double_as_longlong(p[i].x));
-                bad |= p[i].y != 0.0;
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-            bad = __any_sync(0xffffffffu, bad) || best == 0;
-            if (lane == 0) {
-                a.accepted[b] = stop_s;
-                a.tokens[b] = bad ? -1 : 0x7fffffff - (int)(best & 0xffffffffu);
-            }
+            const int first = first_of(stop_s);
+            if (lane == 0) { a.accepted[b] = stop_s; a.tokens[b] = first; }
         }
         return;
     }
     // ---- which drafts are accepted (every block of the cluster finds the same) ----
-    const double inv_t = (double)a.inv_hi + (double)a.inv_lo;
-    for (int j = warp; j < n; j += DR_WARPS) {
-        float top;
-        double sum;
-        join_pieces(a, row0 + j, &top, &sum);
-        const int x = a.drafts[d0 + j];
-        double p = 0.0, q = 1.0;
-        if (x >= 0 && x < a.vocab) {
-            p = exp(((double)a.logits[(long long)(row0 + j) * a.stride + x] - (double)top) * inv_t) / sum;
-            if (a.draft_logits != nullptr) {
-                join_pieces(a, n_target + d0 + j, &top, &sum);
-                q = exp(((double)a.draft_logits[(long long)(d0 + j) * a.draft_stride + x] - (double)top) * inv_t) / sum;
+    const double steps = draft_steps(a);
+    const bool with_q = a.draft_logits != nullptr;
+    for (int j = warp; j <= n; j += DR_WARPS) {
+        // (what does not wait for one another is asked for together)
+        const int x = j < n ? a.drafts[d0 + j] : -1;
+        const bool inside = x >= 0 && x < a.vocab;
+        const float u = j < n ? a.accept_u[d0 + j] : 0.0f;
+        const float at_p = inside ? a.logits[(long long)(row0 + j) * a.stride + x] : 0.0f;
+        const float at_q = inside && with_q ? a.draft_logits[(long long)(d0 + j) * a.draft_stride + x] : 0.0f;
+        const RowSum p = join_pieces(a, row0 + j, table_s);
+        RowSum q{};
+        if (j < n && with_q) q = join_pieces(a, n_target + d0 + j, table_s);
+        if (lane == 0) {
+            if (j < DR_KEPT) { rows_s[j][0] = p; rows_s[j][1] = q; }
+            if (j < n) {
+                const double px = draft_exp(at_p, steps, -(double)p.top * steps, table_s) / p.sum;
+                const double qx = with_q ? draft_exp(at_q, steps, -(double)q.top * steps, table_s) / q.sum : 1.0;
+                // (false for NaN, for a token outside the vocabulary, and for one that the target cannot give)
+                if (!inside || !((double)u * qx < px)) atomicMin(&stop_s, j);
             }
         }
-        // (false for NaN, for a token outside the vocabulary, and for one that the target cannot give)
-        if (lane == 0 && !((double)a.accept_u[d0 + j] * q < p)) atomicMin(&stop_s, j);
     }
     __syncthreads();
     const int stop = stop_s;
     bool less = stop < n;                                    // draw from what q leaves of p
-    const bool with_q = a.draft_logits != nullptr;
-    if (warp == 0) {
-        join_pieces(a, row0 + stop, top_s, all_s);
-    } else if (warp == 1 && less && with_q) {
-        join_pieces(a, n_target + d0 + stop, top_s + 1, all_s + 1);
+    RowSum p, q;
+    if (stop < DR_KEPT) {
+        p = rows_s[stop][0]; q = rows_s[stop][1];
+    } else {
+        p = join_pieces(a, row0 + stop, table_s);
+        q = RowSum{};
+        if (less && with_q) q = join_pieces(a, n_target + d0 + stop, table_s);
     }
-    __syncthreads();
-    const float top_p = top_s[0];
-    const double sum_p = all_s[0];
-    if (!(sum_p > 0.0)) {                                    // no distribution (uniform over the cluster)
+    if (!(p.sum > 0.0)) {                                    // no distribution (uniform over the cluster)
         if (rank == 0 && tid == 0) { a.accepted[b] = stop; a.tokens[b] = -1; }
         return;
     }
-    const float top_q = less && with_q ? top_s[1] : 0.0f;
-    const double inv_p = 1.0 / sum_p, inv_q = less && with_q ? 1.0 / all_s[1] : 0.0;
-    const double steps = draft_steps(a), off_p = -(double)top_p * steps, off_q = -(double)top_q * steps;
+    const double inv_p = 1.0 / p.sum, inv_q = less && with_q ? 1.0 / q.sum : 0.0;
+    const double off_p = -(double)p.top * steps, off_q = -(double)q.top * steps;
     const float* lp = a.logits + (long long)(row0 + stop) * a.stride;
     const float* lq = with_q ? a.draft_logits + (long long)(d0 + (less ? stop : 0)) * a.draft_stride : nullptr;
     const int x = less ? a.drafts[d0 + stop] : -1;
     // what token i weighs
-    auto left = [&](int i, float p, float q) -> double {
-        const double wp = draft_exp(p, steps, off_p, table_s) * inv_p;
+    auto left = [&](int i, float vp, float vq) -> double {
+        const double wp = draft_exp(vp, steps, off_p, table_s) * inv_p;
         if (!less) return wp;
         if (!with_q) return i == x ? 0.0 : wp;
-        return fmax(0.0, wp - draft_exp(q, steps, off_q, table_s) * inv_q);      // (a NaN beside 0: 0)
+        return fmax(0.0, wp - draft_exp(vq, steps, off_q, table_s) * inv_q);      // (a NaN beside 0: 0)
     };
-    // stretches are multiples of 128, a warp's step of four neighbours a lane
-    const int warps = DR_CLUSTER * DR_WARPS;
-    const int each = ((a.vocab + warps - 1) / warps + 127) & ~127;
-    // the four tokens of a lane from i0 on, as far as they are below `to`
-    auto four = [&](int i0, int to, double* w) {
-        float p[4], q[4];
-        if (VEC && i0 + 3 < to) {
+    // stretches are whole steps, a step `wide` times four neighbours a lane
+    const int stretches = blocks * DR_WARPS;
+    const int wide = (a.vocab + stretches * DR_STEPS * 128 - 1) / (stretches * DR_STEPS * 128), step = 128 * wide;
+    const int n_steps = (a.vocab + stretches * step - 1) / (stretches * step);
+    const int each = n_steps * step;
+    // the four tokens of a lane from i0 on, as far as they are below the vocabulary
+    auto four = [&](int i0, double* w) {
+        float vp[4], vq[4];
+        if (VEC && i0 + 3 < a.vocab) {
             const float4 v = *reinterpret_cast<const float4*>(lp + i0);
-            p[0] = v.x; p[1] = v.y; p[2] = v.z; p[3] = v.w;
+            vp[0] = v.x; vp[1] = v.y; vp[2] = v.z; vp[3] = v.w;
             if (less && with_q) {
                 const float4 u = *reinterpret_cast<const float4*>(lq + i0);
-                q[0] = u.x; q[1] = u.y; q[2] = u.z; q[3] = u.w;
+                vq[0] = u.x; vq[1] = u.y; vq[2] = u.z; vq[3] = u.w;
             } else {
-                q[0] = q[1] = q[2] = q[3] = 0.0f;
+                vq[0] = vq[1] = vq[2] = vq[3] = 0.0f;
             }
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                p[e] = i0 + e < to ? lp[i0 + e] : -INFINITY;
-                q[e] = i0 + e < to && less && with_q ? lq[i0 + e] : 0.0f;
+                vp[e] = i0 + e < a.vocab ? lp[i0 + e] : -INFINITY;
+                vq[e] = i0 + e < a.vocab && less && with_q ? lq[i0 + e] : 0.0f;
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = i0 + e < to ? left(i0 + e, p[e], q[e]) : 0.0;
+        for (int e = 0; e < 4; ++e) w[e] = i0 + e < a.vocab ? left(i0 + e, vp[e], vq[e]) : 0.0;
     };
     cluster.sync();                                          // every block runs before another writes to it
+    const int me = rank * DR_WARPS + warp, from = me * each;
     for (int round = 0; ; ++round) {
-        const int me = rank * DR_WARPS + warp;
-        const int from = min(a.vocab, me * each), to = min(a.vocab, from + each);
         double sum = 0.0;
-#pragma unroll 4
-        for (int i = from + 4 * lane; i < to; i += 128) {
-            double w[4];
-            four(i, to, w);
-            sum += (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll 2
+        for (int s = 0; s < n_steps; ++s) {
+            double part = 0.0;
+            for (int k = 0; k < wide; ++k) {
+                const int i0 = from + s * step + k * 128;
+                double w[4] = {0.0, 0.0, 0.0, 0.0};
+                if (i0 < a.vocab) four(i0 + 4 * lane, w);
+                part += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+            part = warp_sum_d(part);
+            if (lane == 0) steps_s[warp][s] = part;
+            sum += part;
         }
-        sum = warp_sum_d(sum);
-        if (lane < DR_CLUSTER) *cluster.map_shared_rank(&sums_s[round][me], lane) = sum;
+        if (lane < blocks) *cluster.map_shared_rank(&sums_s[round][me], lane) = sum;
         cluster.sync();                                      // every block has every sum
         if (sum_of_stretches(sums_s[round]) > 0.0 || !less) break;
         // nothing is left of p (rounding, or a number of 1 or more): from p itself
         less = false;
     }
-    // ---- the first block finds the token ----
-    if (rank == 0 && warp == 0) {
+    // ---- the block whose stretch it is finds the token ----
+    if (warp == 0) {
         const double* sums = sums_s[stop < n && !less ? 1 : 0];
         const double want = (double)a.draw_u[b] * sum_of_stretches(sums);
         // the stretch: the first whose end lies beyond `want`, else the last that holds anything
@@ -394,11 +413,19 @@ __global__ void __launch_bounds__(DR_WARPS * 32) draft_resolve_kernel(DraftArgs 
         for (int e = 0; e < 4; ++e) w[e] = sums[4 * lane + e];
         const Crossing s = find_crossing(w, want, &run);
         const int pick = max(0, s.first >= 0 ? s.first : s.last);
-        const int from = min(a.vocab, pick * each), to = min(a.vocab, from + each);
-        int token = -1, last = -1;
+        if (pick / DR_WARPS != rank) return;
+        // the step of it, the same way, and the token of the step
         run = s.first >= 0 ? s.before_first : s.before_last;
-        for (int i0 = from; i0 < to && token < 0; i0 += 128) {
-            four(i0 + 4 * lane, to, w);
+        const double* parts = steps_s[pick % DR_WARPS];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = 4 * lane + e < n_steps ? parts[4 * lane + e] : 0.0;
+        const Crossing t = find_crossing(w, want, &run);
+        const int in = max(0, t.first >= 0 ? t.first : t.last);
+        run = t.first >= 0 ? t.before_first : t.before_last;
+        int token = -1, last = -1;
+        for (int k = 0; k < wide && token < 0; ++k) {
+            const int i0 = pick * each + in * step + k * 128;
+            four(i0 + 4 * lane, w);
             const Crossing c = find_crossing(w, want, &run);
             if (c.first >= 0) token = i0 + c.first;
             if (c.last >= 0) last = i0 + c.last;
@@ -415,18 +442,22 @@ template <bool VEC> static int drafts_launch(const DraftArgs& a, int rows, cudaS
     if (a.draft_logits != nullptr) mf_launch(draft_pieces_kernel<VEC, true>, grid, dim3(DR_THREADS), 0, stream, a);
     else mf_launch(draft_pieces_kernel<VEC, false>, grid, dim3(DR_THREADS), 0, stream, a);
     if (int e = MF_LAUNCH_CHECK()) return e;
+    // as many blocks a sequence as the GPU holds at once, two an SM
+    int blocks = DR_CLUSTER;
+    while (blocks > 1 && (long long)a.n_seqs * blocks > 2 * mf_sm_count()) blocks >>= 1;
+    if (a.greedy) blocks = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.n_seqs * DR_CLUSTER);
+    cfg.gridDim = dim3(a.n_seqs * blocks);
     cfg.blockDim = dim3(DR_WARPS * 32);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = DR_CLUSTER; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = blocks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = mf_pdl_enabled() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, draft_resolve_kernel<VEC>, a);
+    cudaLaunchKernelEx(&cfg, draft_resolve_kernel<VEC>, a, blocks);
     return MF_LAUNCH_CHECK();
 }
 
