@@ -52,35 +52,44 @@ struct DraftArgs {
     double2* pieces;                                 // [rows][n_pieces]: {maximum, sum}, or {key, NaN seen}
     int n_drafts, n_seqs, vocab, n_pieces;
     float inv_hi, inv_lo;                            // 1 / T = hi + lo (an error in it would tilt every weight)
+    float temperature;
     int greedy;
 };
 
-// exp(d / T) in double to 2e-13 of the result, by the table-driven method (P. T. P. Tang, 1989):
-// d / T = (16 k + j + r) ln 2 / 16 with |r| <= 1/2, so the result is 2^k 2^(j/16) exp(r ln 2 / 16), the
-// last factor its series up to the fifth power.  The table's 16 entries lie in 32 different banks: a warp's
-// look-ups never collide.  0 below exp(-690); NaN stays NaN.  11 operations in double.
-#define DR_TABLE 16
+// exp((logit - top) / T) in double to 2e-12 of the result, by the table-driven method (P. T. P. Tang, 1989):
+// the exponent is (32 k + j + r) ln 2 / 32 with |r| <= 1/2, so the result is 2^k 2^(j/32) exp(r ln 2 / 32), the last
+// factor its series up to the fourth power.  0 below exp(-690) and for -infinity; NaN stays NaN; +infinity
+// against itself counts as nothing.  Ten operations in double, beside which the look-up and the exponent's
+// bits are integer work.
+#define DR_TABLE 32
+struct DraftExp {
+    double steps, off;                               // 32 / (T ln 2), and -top times that
+    float least;                                     // logits up to here weigh nothing
+};
 __device__ __forceinline__ void draft_table(double* table) {
     if (threadIdx.x < DR_TABLE) table[threadIdx.x] = exp2((double)threadIdx.x / DR_TABLE);
 }
-__device__ __forceinline__ double draft_steps(const DraftArgs& a) {       // 16 / (T ln 2)
-    return ((double)a.inv_hi + (double)a.inv_lo) * (16.0 * 1.4426950408889634074);
+__device__ __forceinline__ DraftExp draft_against(const DraftArgs& a, float top) {
+    DraftExp e;
+    e.steps = ((double)a.inv_hi + (double)a.inv_lo) * (DR_TABLE * 1.4426950408889634074);
+    e.off = -(double)top * e.steps;
+    e.least = top - 690.0f * a.temperature;
+    return e;
 }
-// `off` = -top * steps
-__device__ __forceinline__ double draft_exp(float logit, double steps, double off, const double* table) {
-    const double x = fma((double)logit, steps, off);
+__device__ __forceinline__ double draft_exp(float logit, const DraftExp& e, const double* table) {
+    constexpr double L = 0.69314718055994530942 / DR_TABLE;
+    const double x = fma((double)logit, e.steps, e.off);
     const double magic = 6755399441055744.0;                              // 1.5 2^52: the sum's low word is round(x)
     const double shifted = x + magic;
     const int n = __double2loint(shifted);
-    const double z = (x - (shifted - magic)) * (0.69314718055994530942 / 16.0);
-    double q = fma(z, 1.0 / 120.0, 1.0 / 24.0);
-    q = fma(q, z, 1.0 / 6.0);
-    q = fma(q, z, 0.5);
-    q = fma(q, z, 1.0);
-    q = fma(q, z, 1.0);
+    const double r = x - (shifted - magic);
+    double q = fma(r, L * L * L * L / 24.0, L * L * L / 6.0);
+    q = fma(q, r, L * L / 2.0);
+    q = fma(q, r, L);
+    q = fma(q, r, 1.0);
     const double t = table[n & (DR_TABLE - 1)];
-    const double scaled = __hiloint2double(__double2hiint(t) + ((n >> 4) << 20), __double2loint(t));
-    return x < -16000.0 ? 0.0 : q * scaled;
+    const double scaled = __hiloint2double(__double2hiint(t) + ((n >> 5) << 20), __double2loint(t));
+    return logit <= e.least ? 0.0 : q * scaled;
 }
 
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -156,11 +165,11 @@ __global__ void __launch_bounds__(DR_THREADS) draft_pieces_kernel(DraftArgs a) {
     const float m = top == -INFINITY ? 0.0f : top;   // (nothing but -infinity: a sum of 0)
     double sum = 0.0;
     if (EXACT) {
-        const double steps = draft_steps(a), off = -(double)m * steps;
-        double part[2] = {0.0, 0.0};
+        const DraftExp e = draft_against(a, top);
+        double part[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-        for (int i = 0; i < DR_EACH; ++i) part[i & 1] += draft_exp(v[i], steps, off, table_s);
-        sum = part[0] + part[1];
+        for (int i = 0; i < DR_EACH; ++i) part[i & 3] += draft_exp(v[i], e, table_s);
+        sum = (part[0] + part[1]) + (part[2] + part[3]);
     } else {
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -185,19 +194,17 @@ struct RowSum {
 __device__ __forceinline__ RowSum join_pieces(const DraftArgs& a, int row, const double* table) {
     const double2* p = a.pieces + (size_t)row * a.n_pieces;
     const int lane = threadIdx.x & 31;
-    const double steps = draft_steps(a);
     RowSum r;
     r.top = -INFINITY;
     double s = 0.0;
     // (32 pieces are 262,144 tokens: more only beyond that)
     for (int i0 = 0; i0 < a.n_pieces; i0 += 32) {
         const double2 v = i0 + lane < a.n_pieces ? p[i0 + lane] : make_double2((double)-INFINITY, 0.0);
-        const float mine = (float)v.x, top = fmaxf(r.top, warp_max(mine));
-        // a piece of nothing but -infinity has a sum of 0, or NaN if that is among it
-        const double off = -(double)(top == -INFINITY ? 0.0f : top) * steps;
-        const double part = v.y * (mine == -INFINITY ? 1.0 : draft_exp(mine, steps, off, table));
-        if (i0 > 0) s *= r.top == -INFINITY ? 1.0 : draft_exp(r.top, steps, off, table);
-        s += part;
+        const float top = fmaxf(r.top, warp_max((float)v.x));
+        const DraftExp e = draft_against(a, top);
+        // (a piece of nothing but -infinity has a sum of 0, or NaN if that is among it: 0 times it)
+        if (i0 > 0) s *= draft_exp(r.top, e, table);
+        s += v.y * draft_exp((float)v.x, e, table);
         r.top = top;
     }
     s = warp_sum_d(s);
@@ -252,8 +259,9 @@ __device__ __forceinline__ double sum_of_stretches(const double* sums) {
 }
 static_assert(DR_CLUSTER * DR_WARPS == 128, "a lane takes four stretches");
 
-template <bool VEC>
-__global__ void __launch_bounds__(DR_WARPS * 32) draft_resolve_kernel(DraftArgs a, int blocks) {
+// MINB: blocks an SM the registers are cut for (with one, four steps' loads and exponentials are in flight)
+template <bool VEC, int MINB>
+__global__ void __launch_bounds__(DR_WARPS * 32, MINB) draft_resolve_kernel(DraftArgs a, int blocks) {
     namespace cg = cooperative_groups;
     __shared__ double table_s[DR_TABLE];
     __shared__ double sums_s[2][DR_CLUSTER * DR_WARPS];      // the stretches' sums, of every warp of the cluster
@@ -304,7 +312,6 @@ __global__ void __launch_bounds__(DR_WARPS * 32) draft_resolve_kernel(DraftArgs 
         return;
     }
     // ---- which drafts are accepted (every block of the cluster finds the same) ----
-    const double steps = draft_steps(a);
     const bool with_q = a.draft_logits != nullptr;
     for (int j = warp; j <= n; j += DR_WARPS) {
         // (what does not wait for one another is asked for together)
@@ -313,14 +320,15 @@ __global__ void __launch_bounds__(DR_WARPS * 32) draft_resolve_kernel(DraftArgs 
         const float u = j < n ? a.accept_u[d0 + j] : 0.0f;
         const float at_p = inside ? a.logits[(long long)(row0 + j) * a.stride + x] : 0.0f;
         const float at_q = inside && with_q ? a.draft_logits[(long long)(d0 + j) * a.draft_stride + x] : 0.0f;
+        // (both rows' sums side by side)
         const RowSum p = join_pieces(a, row0 + j, table_s);
         RowSum q{};
         if (j < n && with_q) q = join_pieces(a, n_target + d0 + j, table_s);
         if (lane == 0) {
             if (j < DR_KEPT) { rows_s[j][0] = p; rows_s[j][1] = q; }
             if (j < n) {
-                const double px = draft_exp(at_p, steps, -(double)p.top * steps, table_s) / p.sum;
-                const double qx = with_q ? draft_exp(at_q, steps, -(double)q.top * steps, table_s) / q.sum : 1.0;
+                const double px = draft_exp(at_p, draft_against(a, p.top), table_s) / p.sum;
+                const double qx = with_q ? draft_exp(at_q, draft_against(a, q.top), table_s) / q.sum : 1.0;
                 // (false for NaN, for a token outside the vocabulary, and for one that the target cannot give)
                 if (!inside || !((double)u * qx < px)) atomicMin(&stop_s, j);
             }
@@ -341,17 +349,18 @@ __global__ void __launch_bounds__(DR_WARPS * 32) draft_resolve_kernel(DraftArgs 
         if (rank == 0 && tid == 0) { a.accepted[b] = stop; a.tokens[b] = -1; }
         return;
     }
-    const double inv_p = 1.0 / p.sum, inv_q = less && with_q ? 1.0 / q.sum : 0.0;
-    const double off_p = -(double)p.top * steps, off_q = -(double)q.top * steps;
+    // (weights in units of the target's sum: a draw only compares them with one another)
+    const double ratio = less && with_q ? p.sum / q.sum : 0.0;
+    const DraftExp of_p = draft_against(a, p.top), of_q = draft_against(a, q.top);
     const float* lp = a.logits + (long long)(row0 + stop) * a.stride;
     const float* lq = with_q ? a.draft_logits + (long long)(d0 + (less ? stop : 0)) * a.draft_stride : nullptr;
     const int x = less ? a.drafts[d0 + stop] : -1;
     // what token i weighs
     auto left = [&](int i, float vp, float vq) -> double {
-        const double wp = draft_exp(vp, steps, off_p, table_s) * inv_p;
+        const double wp = draft_exp(vp, of_p, table_s);
         if (!less) return wp;
         if (!with_q) return i == x ? 0.0 : wp;
-        return fmax(0.0, wp - draft_exp(vq, steps, off_q, table_s) * inv_q);      // (a NaN beside 0: 0)
+        return fmax(0.0, wp - draft_exp(vq, of_q, table_s) * ratio);      // (a NaN beside 0: 0)
     };
     // stretches are whole steps, a step `wide` times four neighbours a lane
     const int stretches = blocks * DR_WARPS;
@@ -384,8 +393,35 @@ __global__ void __launch_bounds__(DR_WARPS * 32) draft_resolve_kernel(DraftArgs 
     const int me = rank * DR_WARPS + warp, from = me * each;
     for (int round = 0; ; ++round) {
         double sum = 0.0;
-#pragma unroll 2
-        for (int s = 0; s < n_steps; ++s) {
+        int s0 = 0;
+        // four steps at a time where they lie inside the vocabulary: their loads and sums overlap
+        if (VEC && wide == 1)
+            for (; s0 + 4 <= n_steps && from + (s0 + 4) * 128 <= a.vocab; s0 += 4) {
+                float4 vp[4], vq[4];
+                double part[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int i0 = from + (s0 + k) * 128 + 4 * lane;
+                    vp[k] = *reinterpret_cast<const float4*>(lp + i0);
+                    vq[k] = less && with_q ? *reinterpret_cast<const float4*>(lq + i0) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int i0 = from + (s0 + k) * 128 + 4 * lane;
+                    part[k] = (left(i0, vp[k].x, vq[k].x) + left(i0 + 1, vp[k].y, vq[k].y)) +
+                              (left(i0 + 2, vp[k].z, vq[k].z) + left(i0 + 3, vp[k].w, vq[k].w));
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) part[k] += __shfl_xor_sync(0xffffffffu, part[k], o);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (lane == 0) steps_s[warp][s0 + k] = part[k];
+                    sum += part[k];
+                }
+            }
+        for (int s = s0; s < n_steps; ++s) {
             double part = 0.0;
             for (int k = 0; k < wide; ++k) {
                 const int i0 = from + s * step + k * 128;
@@ -442,8 +478,11 @@ template <bool VEC> static int drafts_launch(const DraftArgs& a, int rows, cudaS
     if (a.draft_logits != nullptr) mf_launch(draft_pieces_kernel<VEC, true>, grid, dim3(DR_THREADS), 0, stream, a);
     else mf_launch(draft_pieces_kernel<VEC, false>, grid, dim3(DR_THREADS), 0, stream, a);
     if (int e = MF_LAUNCH_CHECK()) return e;
-    // as many blocks a sequence as the GPU holds at once, two an SM
+    // as many blocks a sequence as the GPU holds at once: one an SM if that is the most a cluster takes, else two.
+    // us, one / two an SM, both launches: 1 sequence of 4 drafts with their logits 21.4 / 23.3, 8 of 4 36.0 / 45.8, 64 of
+    // 4 153 / 142, 64 of 0 to 7 looked up 78 / 70.
     int blocks = DR_CLUSTER;
+    const bool few = (long long)a.n_seqs * blocks <= mf_sm_count();
     while (blocks > 1 && (long long)a.n_seqs * blocks > 2 * mf_sm_count()) blocks >>= 1;
     if (a.greedy) blocks = 1;
     cudaLaunchConfig_t cfg = {};
@@ -457,7 +496,8 @@ template <bool VEC> static int drafts_launch(const DraftArgs& a, int rows, cudaS
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = mf_pdl_enabled() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, draft_resolve_kernel<VEC>, a, blocks);
+    if (few) cudaLaunchKernelEx(&cfg, draft_resolve_kernel<VEC, 1>, a, blocks);
+    else cudaLaunchKernelEx(&cfg, draft_resolve_kernel<VEC, 2>, a, blocks);
     return MF_LAUNCH_CHECK();
 }
 
@@ -479,6 +519,7 @@ extern "C" int mf_verify_drafts(const float* logits, long long stride, const int
     const double inv = a.greedy ? 0.0 : 1.0 / temperature;
     a.inv_hi = (float)inv;
     a.inv_lo = (float)(inv - (double)a.inv_hi);
+    a.temperature = (float)temperature;
     const long long rows = (long long)n_drafts + n_seqs + (a.draft_logits ? n_drafts : 0);
     if (rows * a.n_pieces > 0x7fffffffLL || (long long)n_seqs * DR_CLUSTER > 0x7fffffffLL) return MF_ERR_UNSUPPORTED;
     const bool vec = vocab % 4 == 0 && stride % 4 == 0 && ((uintptr_t)logits & 15) == 0 &&
