@@ -1134,19 +1134,37 @@ def _q8(pages: Q8Pages, n_kv: int, head_dim: int, what: str) -> int:
     return fmt
 
 
-def _here(t: torch.Tensor, what: str) -> None:
-    """Launches go to the current device's stream: the tensors must live there."""
-    if not t.is_cuda:
+# The calls below take a dozen tensors each and run for a few microseconds: every tensor is looked at once
+# (type, device, contiguity, address), libraries' functions are looked up once.
+_functions: Dict[tuple, object] = {}
+
+
+def _fn(library: str, name: str):
+    got = _functions.get((library, name))
+    if got is None:
+        got = _functions[(library, name)] = getattr(_lib(library), name)
+    return got
+
+
+def _here(t: torch.Tensor, what: str) -> int:
+    """The device's index.  Launches go to the current device's stream: the tensors must live there."""
+    device = t.get_device()
+    if device < 0:
         raise KernelError(f"{what}: tensors must live on a CUDA device (there is no CPU path)")
-    if t.device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: the tensors live on {t.device}, which is not the current device")
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: the tensors live on cuda:{device}, which is not the current device")
+    return device
 
 
-def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    _here(first, what)
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise KernelError(f"{what}: tensors on {first.device} and {t.device}")
+def _at(t: torch.Tensor, dtype: torch.dtype, device: int, name: str) -> int:
+    """The address of a contiguous tensor of this type on this device."""
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        raise KernelError(f"{name} must be {dtype}, contiguous and on cuda:{device}, not {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _stream_of(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 _sms_of: Dict[int, int] = {}
@@ -1201,15 +1219,16 @@ def rope_kvstore_q8(qkv: torch.Tensor, positions: torch.Tensor, token_row: torch
     if ring < 0 or ring % PAGE != 0:
         raise KernelError(f"{what}: a ring is whole pages, not {ring} positions")
     _table(page_table, table_stride, seq_end.numel(), what)
-    _same_device(what, qkv, q_out, k_out, v_out, *pages, positions, token_row, seq_end, page_table, inv_freq, status,
-                 bias)
-    _check(_lib("cache_q8").mf_rope_kvstore_q8(
-        _f32(qkv, "qkv"), int(n_partials), _f32(bias, "bias"), _i32(positions, "positions"),
-        _i32(token_row, "token_row"), _i32(seq_end, "seq_end"), _f64(inv_freq, "inv_freq"), _ptr(q_out, "q_out"),
-        _ptr(k_out, "k_out"), _ptr(v_out, "v_out"), _ptr(pages.k, "keys"), _ptr(pages.v, "values"),
-        _ptr(pages.k_scale, "key scales"), _ptr(pages.v_scale, "value scales"), _i32(page_table, "page_table"),
-        int(table_stride), int(ring), pages.k.shape[0], n, n_heads, n_kv, head_dim, int(rotary_dim), int(style),
-        dtype_code(dt), fmt, _i32(status, "status"), _stream()), what)
+    at, f32, i32, codes = _here(qkv, what), torch.float32, torch.int32, pages.k.dtype
+    _check(_fn("cache_q8", "mf_rope_kvstore_q8")(
+        _at(qkv, f32, at, "qkv"), n_partials, None if bias is None else _at(bias, f32, at, "bias"),
+        _at(positions, i32, at, "positions"), _at(token_row, i32, at, "token_row"), _at(seq_end, i32, at, "seq_end"),
+        None if inv_freq is None else _at(inv_freq, torch.float64, at, "inv_freq"), _at(q_out, dt, at, "q_out"),
+        None if k_out is None else _at(k_out, dt, at, "k_out"), None if v_out is None else _at(v_out, dt, at, "v_out"),
+        _at(pages.k, codes, at, "keys"), _at(pages.v, codes, at, "values"), _at(pages.k_scale, f32, at, "key scales"),
+        _at(pages.v_scale, f32, at, "value scales"), _at(page_table, i32, at, "page_table"), table_stride, ring,
+        pages.k.shape[0], n, n_heads, n_kv, head_dim, rotary_dim, style, dtype_code(dt), fmt,
+        _at(status, i32, at, "status"), _stream_of(at)), what)
 
 
 def read_pages_q8(pages: Q8Pages, page_table: torch.Tensor, table_stride: int, ring: int, seq_end: torch.Tensor,
@@ -1230,7 +1249,7 @@ def read_pages_q8(pages: Q8Pages, page_table: torch.Tensor, table_stride: int, r
     want = rows * table_stride * n_kv * PAGE * head_dim
     if k_out.dtype != v_out.dtype or k_out.numel() != want or v_out.numel() != want:
         raise KernelError(f"{what}: the outputs must be [rows * table_stride, {n_kv}, {PAGE}, {head_dim}] of one type")
-    _same_device(what, *pages, page_table, seq_end, k_out, v_out, status)
+    _here(k_out, what)
     _read_pages_q8(pages, fmt, page_table, table_stride, table_stride, ring, seq_end, k_out, v_out, status, fill, False)
 
 
@@ -1239,12 +1258,13 @@ def _read_pages_q8(pages: Q8Pages, fmt: int, page_table: torch.Tensor, table_str
                    for_attention: bool) -> None:
     """``out_stride`` pages a row in the output (behind the table's: zeros).  ``for_attention``: a position whose
     key or value is NaN becomes a key of NaN with a value of zeros."""
-    _check(_lib("cache_q8").mf_read_pages_q8(
-        _ptr(pages.k, "keys"), _ptr(pages.v, "values"), _ptr(pages.k_scale, "key scales"),
-        _ptr(pages.v_scale, "value scales"), _i32(page_table, "page_table"), int(table_stride),
-        int(out_stride), int(ring), pages.k.shape[0], _i32(seq_end, "seq_end"), _ptr(k_out, "k_out"),
-        _ptr(v_out, "v_out"), seq_end.numel(), pages.k.shape[1], pages.k.shape[3], dtype_code(k_out.dtype), fmt,
-        1 if fill else 0, 1 if for_attention else 0, _i32(status, "status"), _stream()), "read_pages_q8")
+    at, f32, i32, codes, dt = k_out.get_device(), torch.float32, torch.int32, pages.k.dtype, k_out.dtype
+    _check(_fn("cache_q8", "mf_read_pages_q8")(
+        _at(pages.k, codes, at, "keys"), _at(pages.v, codes, at, "values"), _at(pages.k_scale, f32, at, "key scales"),
+        _at(pages.v_scale, f32, at, "value scales"), _at(page_table, i32, at, "page_table"), table_stride, out_stride,
+        ring, pages.k.shape[0], _at(seq_end, i32, at, "seq_end"), _at(k_out, dt, at, "k_out"),
+        _at(v_out, dt, at, "v_out"), seq_end.numel(), pages.k.shape[1], pages.k.shape[3], dtype_code(dt), fmt,
+        1 if fill else 0, 1 if for_attention else 0, _at(status, i32, at, "status"), _stream_of(at)), "read_pages_q8")
 
 
 _Q8_PLANS: Dict[tuple, tuple] = {}
@@ -1254,7 +1274,7 @@ def attention_q8_plan(n_tokens: int, n_rows: int, max_row_tokens: int, span: int
                       head_dim: int, dtype: torch.dtype) -> tuple[int, int]:
     """(floats of scratch, kernels) that attention over 8-bit pages takes; ``span``: the most positions that
     the queries of a row see."""
-    key = (torch.cuda.current_device(), n_tokens, n_rows, max_row_tokens, span, n_heads, n_kv, head_dim, dtype)
+    key = (torch._C._cuda_getDevice(), n_tokens, n_rows, max_row_tokens, span, n_heads, n_kv, head_dim, dtype)
     got = _Q8_PLANS.get(key)
     if got is None:
         kernels = c_int(0)
@@ -1316,14 +1336,14 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
     if not math.isfinite(scale):
         raise KernelError(f"{what}: the scale must be finite")
     _table(page_table, table_stride, rows, what)
-    _same_device(what, q, *pages, cu_seqlens, seq_end, page_table, out, status)
+    at, f32, i32, codes, dt = _here(q, what), torch.float32, torch.int32, pages.k.dtype, q.dtype
     if tokens == 0 or rows == 0:
         return
-    span = int(max_end)
+    span = max_end
     if window > 0:                    # from a page's border on
-        span = min(span, window + int(max_row_tokens) + PAGE - 1)
-    if q.dtype == torch.bfloat16 and head_dim in (64, 128) and q8_reads_back(
-            tokens, rows, int(max_row_tokens), span, n_heads, n_kv, head_dim, sm_count(q.device)):
+        span = min(span, window + max_row_tokens + PAGE - 1)
+    if max_row_tokens >= 32 and dt is torch.bfloat16 and head_dim in (64, 128) and q8_reads_back(
+            tokens, rows, max_row_tokens, span, n_heads, n_kv, head_dim, sm_count(q.device)):
         # pages of the rows read back, as many rows at a time as the scratch takes; a tile of the kernel is
         # two pages, so a row has an even number of them (the last one zeros where there is none)
         wide = table_stride + (table_stride & 1)
@@ -1339,14 +1359,15 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
             attention_prefill_tc_paged(q, k, v, cu_seqlens[first:last + 1], ends, places, wide, ring, out, last - first,
                                        int(max_row_tokens), n_heads, n_kv, head_dim, int(window), float(scale), status)
         return
-    floats, kernels = attention_q8_plan(tokens, rows, int(max_row_tokens), span, n_heads, n_kv, head_dim, q.dtype)
-    partial = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    _check(_lib("attention_q8").mf_attention_q8(
-        _ptr(q, "q"), _ptr(pages.k, "keys"), _ptr(pages.v, "values"), _ptr(pages.k_scale, "key scales"),
-        _ptr(pages.v_scale, "value scales"), _i32(cu_seqlens, "cu_seqlens"), _i32(seq_end, "seq_end"),
-        _i32(page_table, "page_table"), int(table_stride), int(ring), pages.k.shape[0], _ptr(out, "out"),
-        _f32(partial, "partial"), tokens, rows, int(max_row_tokens), span, n_heads, n_kv, head_dim,
-        int(window), float(scale), dtype_code(q.dtype), fmt, _i32(status, "status"), _stream()), what, kernels)
+    floats, kernels = attention_q8_plan(tokens, rows, max_row_tokens, span, n_heads, n_kv, head_dim, dt)
+    partial = torch.empty(floats, dtype=f32, device=q.device) if floats else None
+    _check(_fn("attention_q8", "mf_attention_q8")(
+        _at(q, dt, at, "q"), _at(pages.k, codes, at, "keys"), _at(pages.v, codes, at, "values"),
+        _at(pages.k_scale, f32, at, "key scales"), _at(pages.v_scale, f32, at, "value scales"),
+        _at(cu_seqlens, i32, at, "cu_seqlens"), _at(seq_end, i32, at, "seq_end"),
+        _at(page_table, i32, at, "page_table"), table_stride, ring, pages.k.shape[0], _at(out, dt, at, "out"),
+        None if partial is None else partial.data_ptr(), tokens, rows, max_row_tokens, span, n_heads, n_kv, head_dim,
+        window, scale, dtype_code(dt), fmt, _at(status, i32, at, "status"), _stream_of(at)), what, kernels)
 
 
 # ---------------------------------------------------------------------------------------
@@ -2607,16 +2628,17 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.T
         raise KernelError(f"{what}: sizes do not fit {n} drafts of {rows} sequences")
     if not (math.isfinite(temperature) and temperature >= 0.0):
         raise KernelError(f"{what}: temperature must be finite and not negative")
-    _same_device(what, logits, drafts, cu_drafts, draft_logits, accept_u, draw_u, accepted, tokens)
+    at, f32, i32 = _here(logits, what), torch.float32, torch.int32
+    if draft_logits is not None and draft_logits.get_device() != at:
+        raise KernelError(f"{what}: the drafts' logits must live on cuda:{at}")
     if rows == 0:
         return
-    lib = _lib("drafts")
     # two numbers for every piece of a row
-    pieces = torch.empty(2 * (logits.shape[0] + (n if draft_logits is not None else 0)) * lib.mf_draft_pieces(vocab),
-                         dtype=torch.float64, device=logits.device)
-    _check(lib.mf_verify_drafts(
-        logits.data_ptr(), logits.stride(0), _i32(drafts, "drafts"), _i32(cu_drafts, "cu_drafts"),
+    pieces = torch.empty(2 * (logits.shape[0] + (n if draft_logits is not None else 0)) *
+                         _fn("drafts", "mf_draft_pieces")(vocab), dtype=torch.float64, device=logits.device)
+    _check(_fn("drafts", "mf_verify_drafts")(
+        logits.data_ptr(), logits.stride(0), _at(drafts, i32, at, "drafts"), _at(cu_drafts, i32, at, "cu_drafts"),
         None if draft_logits is None else draft_logits.data_ptr(),
-        0 if draft_logits is None else draft_logits.stride(0), _f32(accept_u, "accept_u"), _f32(draw_u, "draw_u"),
-        float(temperature), _i32(accepted, "accepted"), _i32(tokens, "tokens"), pieces.data_ptr(), n, rows, vocab,
-        _stream()), what, 2)
+        0 if draft_logits is None else draft_logits.stride(0), _at(accept_u, f32, at, "accept_u"),
+        _at(draw_u, f32, at, "draw_u"), temperature, _at(accepted, i32, at, "accepted"), _at(tokens, i32, at, "tokens"),
+        pieces.data_ptr(), n, rows, vocab, _stream_of(at)), what, 2)
