@@ -777,13 +777,14 @@ __global__ void __launch_bounds__(AQ_JOIN_WARPS * 32) attention_q8_join_kernel(A
 // Any head size that is a multiple of 16 up to 256, float32 or bfloat16 queries, in float32 on the
 // FP32 pipe (the true 32-bit path).  A block takes up to eight matrix rows of one key/value head; 32
 // keys at a time are turned into float32 codes in shared memory once for all of them, lanes are keys
-// in the scores and dimensions in the sums.  Bound by the shared-memory reads of the products.
+// in the scores and dimensions in the sums; a warp's two rows share what it reads of keys and values.  Bound by
+// the shared-memory reads of the products.  ND: 32 dimensions a lane has one of, rounded up to 1, 2, 4 or 8.
 // ------------------------------------------------------------------------------------------
 #define AG_WARPS 4
 #define AG_ROWS 8
 #define AG_KEYS 32
 
-template <typename T, int FMT>
+template <typename T, int FMT, int ND>
 __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(AttnQ8Args a) {
     extern __shared__ __align__(16) uint8_t ag_smem[];
     pdl_launch_dependents();
@@ -813,7 +814,9 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
         q_s[i] = to_f32(((const T*)a.q)[((size_t)(tok0 + token) * a.n_heads + head) * hd + d]) * a.scale;
     }
     constexpr int RW = AG_ROWS / AG_WARPS;                 // rows a warp
-    constexpr int ND = 256 / 32;
+    static_assert(RW == 2, "a warp's weights are read as pairs");
+    // rows that are not there multiply zeros
+    for (int i = tid + rows * hd; i < AG_ROWS * hd; i += AG_WARPS * 32) q_s[i] = 0.0f;
     float m_r[RW], l_r[RW], acc[RW][ND];
     int lo_w[RW], hi_w[RW];
 #pragma unroll
@@ -853,37 +856,54 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
         if (tid < AG_KEYS) ks_s[tid] = a.k_scales[at + tid];
         else if (tid < 2 * AG_KEYS) vs_s[tid - AG_KEYS] = a.v_scales[at + tid - AG_KEYS];
         __syncthreads();
+        const int j = j0 + lane;
+        bool seen[RW], any = false;
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
-            const int r = warp * RW + i, j = j0 + lane;
-            const bool seen = j >= max(lo_w[i], lo) && j < min(hi_w[i], hi);
-            if (!__any_sync(0xffffffffu, seen)) continue;
-            const float* kr = k_s + lane * hs;
-            const float* qr = q_s + r * hd;
-            float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
-            for (int d = 0; d < hd; d += 4) {
-                const float4 q4 = *reinterpret_cast<const float4*>(qr + d);
-                s0 = fmaf(q4.x, kr[d], s0); s1 = fmaf(q4.y, kr[d + 1], s1);
-                s2 = fmaf(q4.z, kr[d + 2], s2); s3 = fmaf(q4.w, kr[d + 3], s3);
+            seen[i] = j >= max(lo_w[i], lo) && j < min(hi_w[i], hi);
+            any |= seen[i];
+        }
+        if (!__any_sync(0xffffffffu, any)) continue;
+        const float* kr = k_s + lane * hs;
+        const float* qr = q_s + warp * RW * hd;
+        float dot[RW][4];
+#pragma unroll
+        for (int i = 0; i < RW; ++i) dot[i][0] = dot[i][1] = dot[i][2] = dot[i][3] = 0.0f;
+#pragma unroll 4
+        for (int d = 0; d < hd; d += 4) {
+            const float k0 = kr[d], k1 = kr[d + 1], k2 = kr[d + 2], k3 = kr[d + 3];
+#pragma unroll
+            for (int i = 0; i < RW; ++i) {
+                const float4 q4 = *reinterpret_cast<const float4*>(qr + i * hd + d);
+                dot[i][0] = fmaf(q4.x, k0, dot[i][0]); dot[i][1] = fmaf(q4.y, k1, dot[i][1]);
+                dot[i][2] = fmaf(q4.z, k2, dot[i][2]); dot[i][3] = fmaf(q4.w, k3, dot[i][3]);
             }
-            const float s = seen ? ((s0 + s1) + (s2 + s3)) * ks_s[lane] : AQ_NEG;
+        }
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            const float s = seen[i] ? ((dot[i][0] + dot[i][1]) + (dot[i][2] + dot[i][3])) * ks_s[lane] : AQ_NEG;
             const float top = fmaxf(m_r[i], warp_max(s));
             const float m_use = top == AQ_NEG ? 0.0f : top;
             const float f = expf(m_r[i] - m_use), p = expf(s - m_use);
             l_r[i] = l_r[i] * f + warp_sum(p);
             m_r[i] = top;
-            p_s[r * AG_KEYS + lane] = seen ? p * vs_s[lane] : 0.0f;
-            __syncwarp();
+            p_s[(warp * AG_KEYS + lane) * RW + i] = seen[i] ? p * vs_s[lane] : 0.0f;
 #pragma unroll
             for (int d = 0; d < ND; ++d) acc[i][d] *= f;
-            for (int jj = 0; jj < AG_KEYS; ++jj) {
-                const float w = p_s[r * AG_KEYS + jj];
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    if (lane + 32 * d < hd) acc[i][d] = fmaf(w, v_s[jj * hd + lane + 32 * d], acc[i][d]);
-            }
-            __syncwarp();
         }
+        __syncwarp();
+#pragma unroll 8
+        for (int jj = 0; jj < AG_KEYS; ++jj) {
+            const float2 w = *reinterpret_cast<const float2*>(p_s + (warp * AG_KEYS + jj) * RW);
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                if (32 * d + 32 <= hd || lane + 32 * d < hd) {
+                    const float v = v_s[jj * hd + lane + 32 * d];
+                    acc[0][d] = fmaf(w.x, v, acc[0][d]);
+                    acc[1][d] = fmaf(w.y, v, acc[1][d]);
+                }
+        }
+        __syncwarp();
     }
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
@@ -983,7 +1003,7 @@ static AqPlan aq_plan(int n_tokens, int n_rows, int max_row_tokens, int span, in
     const int pages = span <= 0 ? 1 : (span + MF_PAGE - 1) / MF_PAGE, sms = mf_sm_count();
     if (!aq_on_tensor_cores(hd, dtype)) {
         long long splits = 3LL * sms / items;
-        if (splits > (pages + 3) / 4) splits = (pages + 3) / 4;          // 256 keys a split at least
+        if (splits > pages) splits = pages;
         if (splits > AQ_MAX_SPLITS) splits = AQ_MAX_SPLITS;
         p.splits = splits < 1 ? 1 : (int)splits;
         p.floats = p.splits > 1 ? (long long)n_tokens * n_heads * p.splits * (hd + 2) : 0;
@@ -1048,20 +1068,26 @@ static int launch_mma(const AttnQ8Args& a, int items, int splits, cudaStream_t s
            : splits == 1 ? launch_mma_as<HD, FMT, NT, KT, AQ_WHOLE, STAGES, minb>(a, items, 0, stream)
                          : launch_mma_as<HD, FMT, NT, KT, AQ_SPLIT, STAGES, minb>(a, items, 0, stream);
 }
-template <typename T, int FMT> static int launch_generic(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
+template <typename T, int FMT, int ND> static int launch_generic_as(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
     const int smem = (AG_KEYS * (2 * a.hd + 1) + AG_ROWS * a.hd + 2 * AG_KEYS + AG_ROWS * AG_KEYS) * 4;
-    constexpr int most = (AG_KEYS * (2 * 256 + 1) + AG_ROWS * 256 + 2 * AG_KEYS + AG_ROWS * AG_KEYS) * 4;
+    constexpr int hd = 32 * ND, most = (AG_KEYS * (2 * hd + 1) + AG_ROWS * hd + 2 * AG_KEYS + AG_ROWS * AG_KEYS) * 4;
     static bool opened[AQ_MAX_DEVICES] = {};
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
     if (dev < 0 || dev >= AQ_MAX_DEVICES || !opened[dev]) {
-        if (cudaError_t e = cudaFuncSetAttribute(attention_q8_generic_kernel<T, FMT>,
+        if (cudaError_t e = cudaFuncSetAttribute(attention_q8_generic_kernel<T, FMT, ND>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, most))
             return (int)e;
         if (dev >= 0 && dev < AQ_MAX_DEVICES) opened[dev] = true;
     }
-    mf_launch(attention_q8_generic_kernel<T, FMT>, grid, dim3(AG_WARPS * 32), smem, stream, a);
+    mf_launch(attention_q8_generic_kernel<T, FMT, ND>, grid, dim3(AG_WARPS * 32), smem, stream, a);
     return MF_LAUNCH_CHECK();
+}
+template <typename T, int FMT> static int launch_generic(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
+    return a.hd <= 32   ? launch_generic_as<T, FMT, 1>(a, grid, stream)
+           : a.hd <= 64 ? launch_generic_as<T, FMT, 2>(a, grid, stream)
+           : a.hd <= 128 ? launch_generic_as<T, FMT, 4>(a, grid, stream)
+                         : launch_generic_as<T, FMT, 8>(a, grid, stream);
 }
 
 // The scratch of a call in floats; `kernels`: how many it launches.
