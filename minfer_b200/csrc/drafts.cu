@@ -16,12 +16,17 @@
 // A row that holds a NaN, or nothing above -infinity (or, for T > 0, +infinity), is no distribution: its draft
 // is not accepted and the token is -1.
 //
-// Two launches.  The first reads every row once: the maximum and sum of a piece of 8,192 logits, which stay
-// in registers between the two (bound by bytes).  The second joins the pieces, decides, and
-// passes over the one row that the token comes from: a cluster of up to eight blocks a sequence, every warp a
-// contiguous stretch of the vocabulary, whose sums all blocks see; the block whose stretch holds the answer has
-// kept that stretch's sums in steps of 128 tokens, and goes through one step again (through the whole
-// stretch, a step after the other: 25 us more).
+// Three launches.  The first reads every row once: the maximum and sum of a piece of 8,192 logits, which stay
+// in registers between the two.  The second joins the pieces, decides (every block of a sequence finds the
+// same) and passes over the one row that the token comes from: a warp takes steps of 128 tokens and leaves
+// their sums.  The third finds the step that holds the answer and goes through it again.  (The second and
+// third as one, a cluster of eight blocks a sequence: 21 us for one sequence with four drafts over 152,064
+// tokens where this takes 14, since eight SMs form 300,000 exponentials in double; 70 us for 64 of them
+// where this takes 57.)  Of those 57 us the first launch is some 33, 5.9 TB/s of its 195 MB; the second forms
+// ten million exponentials in double, twenty instructions each, and is bound by their latency and issue: 20 us
+// with the 32 warps an SM that 64 registers leave room for and two steps in flight, 24 with 16 warps and four.
+// Where the drafts have distributions of their own, all rows' exponentials are double: 129 us of 64 sequences.
+// One sequence is bound by the latency of its three launches.
 //
 // The token has to be the definition's: a running sum over 150,000 tokens has a border within 7e-6 of any
 // number, and within 1e-8 of one number in 300.  So everything that a draw compares is double, the
@@ -29,15 +34,16 @@
 // is one of float32 exponentials, kept in double.
 #include "common.cuh"
 
-#include <cooperative_groups.h>
-
 #define DR_THREADS 256
 #define DR_EACH 32                                   // logits a thread of the first launch holds
 #define DR_PIECE (DR_THREADS * DR_EACH)
-#define DR_CLUSTER 8                                 // most blocks a sequence
-#define DR_WARPS 16
-#define DR_STEPS 64                                  // most steps of a stretch
+#define DR_WARPS 8                                   // of the second launch's blocks
+#define DR_HELD 4                                    // of those an SM holds at once
+#define DR_MOST 128                                  // most of them a sequence
+#define DR_AHEAD 2                                   // steps that a warp has in flight
+#define DR_STEP 128                                  // tokens of a step: four neighbours a lane
 #define DR_KEPT 32                                   // places whose maximum and sum a block keeps
+#define DR_PICK 512                                  // threads of the third launch's blocks
 
 struct DraftArgs {
     const float* logits;                             // [n_drafts + n_seqs] rows
@@ -50,8 +56,12 @@ struct DraftArgs {
     int* accepted;
     int* tokens;
     double2* pieces;                                 // [rows][n_pieces]: {maximum, sum}, or {key, NaN seen}
+    double* sums;                                    // [n_seqs][n_steps] of the row that the token comes from
+    struct DraftCase* cases;                         // [n_seqs]
+    int n_steps;
     int n_drafts, n_seqs, vocab, n_pieces;
-    float inv_hi, inv_lo;                            // 1 / T = hi + lo (an error in it would tilt every weight)
+    double base2;                                    // log2(e) / T
+    float base2_hi, base2_lo;                        // their sum is that (an error in it would tilt every weight)
     float temperature;
     int greedy;
 };
@@ -71,7 +81,7 @@ __device__ __forceinline__ void draft_table(double* table) {
 }
 __device__ __forceinline__ DraftExp draft_against(const DraftArgs& a, float top) {
     DraftExp e;
-    e.steps = ((double)a.inv_hi + (double)a.inv_lo) * (DR_TABLE * 1.4426950408889634074);
+    e.steps = a.base2 * DR_TABLE;
     e.off = -(double)top * e.steps;
     e.least = top - 690.0f * a.temperature;
     return e;
@@ -98,9 +108,11 @@ __device__ __forceinline__ double warp_sum_d(double v) {
     return v;
 }
 __device__ __forceinline__ float weight_of(float logit, float top, const DraftArgs& a) {
-    // (infinity times a residue of 1 / T would be NaN; a NaN stays)
-    const float apart = logit - top, d = apart < -1e30f ? -1e30f : apart;
-    return expf(fmaf(d, a.inv_hi, d * a.inv_lo));
+    // (infinity times a residue would be NaN, so what is far below is brought near; a NaN stays)
+    float d, w;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(logit - top), "f"(-3e38f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf(d, a.base2_hi, d * a.base2_lo)));
+    return w;
 }
 // larger values first, then lower indices; -0 and +0 are one value
 __device__ __forceinline__ unsigned long long place_key(float v, int index) {
@@ -249,42 +261,97 @@ __device__ __forceinline__ Crossing find_crossing(const double* w, double want, 
     *run += __shfl_sync(0xffffffffu, upto, 31);
     return c;
 }
-// the sum of the cluster's stretches, the same in every warp
-__device__ __forceinline__ double sum_of_stretches(const double* sums) {
-    const int lane = threadIdx.x & 31;
-    double s = 0.0;
-#pragma unroll
-    for (int i = 0; i < DR_CLUSTER * DR_WARPS / 32; ++i) s += sums[lane * (DR_CLUSTER * DR_WARPS / 32) + i];
-    return warp_sum_d(s);
-}
-static_assert(DR_CLUSTER * DR_WARPS == 128, "a lane takes four stretches");
+// What the second launch has decided about a sequence, for the third.
+struct DraftCase {
+    double ratio;                                    // the target's sum over the draft's, where that is taken off
+    float top_p, top_q;
+    int stop;                                        // drafts accepted; -1: nothing is left to do
+    int less;                                        // draw from what q leaves of p
+};
 
-// MINB: blocks an SM the registers are cut for (with one, four steps' loads and exponentials are in flight)
-template <bool VEC, int MINB>
-__global__ void __launch_bounds__(DR_WARPS * 32, MINB) draft_resolve_kernel(DraftArgs a, int blocks) {
-    namespace cg = cooperative_groups;
+// The weights of the row that a token comes from, in units of the target's sum (a draw only compares
+// them with one another).
+struct DraftRow {
+    const float *lp, *lq;
+    DraftExp of_p, of_q;
+    double ratio;
+    int x, vocab;
+    __device__ __forceinline__ DraftRow(const DraftArgs& a, int b, int d0, const DraftCase& c) {
+        const bool less = c.less != 0, with_q = a.draft_logits != nullptr;
+        lp = a.logits + (long long)(d0 + b + c.stop) * a.stride;
+        lq = less && with_q ? a.draft_logits + (long long)(d0 + c.stop) * a.draft_stride : nullptr;
+        of_p = draft_against(a, c.top_p);
+        of_q = draft_against(a, c.top_q);
+        ratio = c.ratio;
+        x = less && !with_q ? a.drafts[d0 + c.stop] : -1;
+        vocab = a.vocab;
+    }
+    // the weights of a lane's four tokens from i0 on (a NaN that q brings: 0)
+    __device__ __forceinline__ void weights(int i0, const float* vp, const float* vq, const double* table,
+                                            double* w) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = draft_exp(vp[e], of_p, table);
+        if (lq != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = fmax(0.0, w[e] - draft_exp(vq[e], of_q, table) * ratio);
+        } else if (x >= i0 && x < i0 + 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i0 + e == x) w[e] = 0.0;
+        }
+    }
+    __device__ __forceinline__ double weight(int i0, const float* vp, const float* vq, const double* table) const {
+        double w[4];
+        weights(i0, vp, vq, table, w);
+        return (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    // a lane's four tokens from i0 on, as far as they are in the vocabulary
+    template <bool VEC> __device__ __forceinline__ void load(int i0, float* vp, float* vq) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vp[e] = vq[e] = -INFINITY;
+        if (VEC) {                                   // (a multiple of 4 tokens)
+            if (i0 < vocab) {
+                const float4 v = *reinterpret_cast<const float4*>(lp + i0);
+                vp[0] = v.x; vp[1] = v.y; vp[2] = v.z; vp[3] = v.w;
+                if (lq != nullptr) {
+                    const float4 u = *reinterpret_cast<const float4*>(lq + i0);
+                    vq[0] = u.x; vq[1] = u.y; vq[2] = u.z; vq[3] = u.w;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i0 + e < vocab) {
+                    vp[e] = lp[i0 + e];
+                    if (lq != nullptr) vq[e] = lq[i0 + e];
+                }
+        }
+    }
+};
+
+template <bool VEC>
+__global__ void __launch_bounds__(DR_WARPS * 32, DR_HELD) draft_sums_kernel(DraftArgs a, int blocks) {
     __shared__ double table_s[DR_TABLE];
-    __shared__ double sums_s[2][DR_CLUSTER * DR_WARPS];      // the stretches' sums, of every warp of the cluster
-    __shared__ double steps_s[DR_WARPS][DR_STEPS];           // this block's stretches, step by step
     __shared__ RowSum rows_s[DR_KEPT][2];                    // of the first places: target, draft
     __shared__ int stop_s;
     draft_table(table_s);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = blockIdx.x % blocks, b = blockIdx.x / blocks;
-    if (tid < 2 * DR_CLUSTER * DR_WARPS) sums_s[0][tid] = 0.0;
     pdl_prologue();
-    cg::cluster_group cluster = cg::this_cluster();
-    const int d0 = a.cu[b], n = a.cu[b + 1] - d0;
-    const bool fits = d0 >= 0 && n >= 0 && d0 + n <= a.n_drafts;       // (uniform over the cluster)
-    const int row0 = d0 + b, n_target = a.n_drafts + a.n_seqs;
-    if (!fits) {
-        if (rank == 0 && tid == 0) { a.accepted[b] = 0; a.tokens[b] = -1; }
-        return;
-    }
+    const int d0 = a.cu[b], end = a.cu[b + 1];
+    // the sequence is done: so many drafts, this token
+    auto answer = [&](int accepted, int token) {
+        if (rank == 0 && tid == 0) {
+            a.accepted[b] = accepted;
+            a.tokens[b] = token;
+            a.cases[b].stop = -1;
+        }
+    };
+    if (d0 < 0 || end < d0 || end > a.n_drafts) { answer(0, -1); return; }
+    const int n = end - d0, row0 = d0 + b, n_target = a.n_drafts + a.n_seqs;
     if (tid == 0) stop_s = n;
     __syncthreads();
     if (a.greedy) {
-        if (rank != 0) return;                               // (no block of this cluster waits for another)
         // the first maximum of place j, -1 if there is none
         auto first_of = [&](int j) {
             const double2* p = a.pieces + (size_t)(row0 + j) * a.n_pieces;
@@ -305,13 +372,10 @@ __global__ void __launch_bounds__(DR_WARPS * 32, MINB) draft_resolve_kernel(Draf
             if (lane == 0 && (first < 0 || first != a.drafts[d0 + j])) atomicMin(&stop_s, j);
         }
         __syncthreads();
-        if (warp == 0) {
-            const int first = first_of(stop_s);
-            if (lane == 0) { a.accepted[b] = stop_s; a.tokens[b] = first; }
-        }
+        if (warp == 0) answer(stop_s, first_of(stop_s));
         return;
     }
-    // ---- which drafts are accepted (every block of the cluster finds the same) ----
+    // ---- which drafts are accepted ----
     const bool with_q = a.draft_logits != nullptr;
     for (int j = warp; j <= n; j += DR_WARPS) {
         // (what does not wait for one another is asked for together)
@@ -320,156 +384,135 @@ __global__ void __launch_bounds__(DR_WARPS * 32, MINB) draft_resolve_kernel(Draf
         const float u = j < n ? a.accept_u[d0 + j] : 0.0f;
         const float at_p = inside ? a.logits[(long long)(row0 + j) * a.stride + x] : 0.0f;
         const float at_q = inside && with_q ? a.draft_logits[(long long)(d0 + j) * a.draft_stride + x] : 0.0f;
-        // (both rows' sums side by side)
         const RowSum p = join_pieces(a, row0 + j, table_s);
         RowSum q{};
         if (j < n && with_q) q = join_pieces(a, n_target + d0 + j, table_s);
         if (lane == 0) {
             if (j < DR_KEPT) { rows_s[j][0] = p; rows_s[j][1] = q; }
             if (j < n) {
-                const double px = draft_exp(at_p, draft_against(a, p.top), table_s) / p.sum;
-                const double qx = with_q ? draft_exp(at_q, draft_against(a, q.top), table_s) / q.sum : 1.0;
-                // (false for NaN, for a token outside the vocabulary, and for one that the target cannot give)
-                if (!inside || !((double)u * qx < px)) atomicMin(&stop_s, j);
+                // u q(x) < p(x), the two sums multiplied out (false for NaN, for a token outside the
+                // vocabulary, and for one that the target cannot give)
+                const double ep = draft_exp(at_p, draft_against(a, p.top), table_s);
+                const double eq = with_q ? draft_exp(at_q, draft_against(a, q.top), table_s) : 1.0;
+                if (!inside || !((double)u * eq * p.sum < ep * (with_q ? q.sum : 1.0))) atomicMin(&stop_s, j);
             }
         }
     }
     __syncthreads();
     const int stop = stop_s;
-    bool less = stop < n;                                    // draw from what q leaves of p
+    DraftCase c;
+    c.stop = stop;
+    c.less = stop < n;
     RowSum p, q;
     if (stop < DR_KEPT) {
         p = rows_s[stop][0]; q = rows_s[stop][1];
     } else {
         p = join_pieces(a, row0 + stop, table_s);
         q = RowSum{};
-        if (less && with_q) q = join_pieces(a, n_target + d0 + stop, table_s);
+        if (c.less && with_q) q = join_pieces(a, n_target + d0 + stop, table_s);
     }
-    if (!(p.sum > 0.0)) {                                    // no distribution (uniform over the cluster)
-        if (rank == 0 && tid == 0) { a.accepted[b] = stop; a.tokens[b] = -1; }
-        return;
-    }
-    // (weights in units of the target's sum: a draw only compares them with one another)
-    const double ratio = less && with_q ? p.sum / q.sum : 0.0;
-    const DraftExp of_p = draft_against(a, p.top), of_q = draft_against(a, q.top);
-    const float* lp = a.logits + (long long)(row0 + stop) * a.stride;
-    const float* lq = with_q ? a.draft_logits + (long long)(d0 + (less ? stop : 0)) * a.draft_stride : nullptr;
-    const int x = less ? a.drafts[d0 + stop] : -1;
-    // what token i weighs
-    auto left = [&](int i, float vp, float vq) -> double {
-        const double wp = draft_exp(vp, of_p, table_s);
-        if (!less) return wp;
-        if (!with_q) return i == x ? 0.0 : wp;
-        return fmax(0.0, wp - draft_exp(vq, of_q, table_s) * ratio);      // (a NaN beside 0: 0)
-    };
-    // stretches are whole steps, a step `wide` times four neighbours a lane
-    const int stretches = blocks * DR_WARPS;
-    const int wide = (a.vocab + stretches * DR_STEPS * 128 - 1) / (stretches * DR_STEPS * 128), step = 128 * wide;
-    const int n_steps = (a.vocab + stretches * step - 1) / (stretches * step);
-    const int each = n_steps * step;
-    // the four tokens of a lane from i0 on, as far as they are below the vocabulary
-    auto four = [&](int i0, double* w) {
-        float vp[4], vq[4];
-        if (VEC && i0 + 3 < a.vocab) {
-            const float4 v = *reinterpret_cast<const float4*>(lp + i0);
-            vp[0] = v.x; vp[1] = v.y; vp[2] = v.z; vp[3] = v.w;
-            if (less && with_q) {
-                const float4 u = *reinterpret_cast<const float4*>(lq + i0);
-                vq[0] = u.x; vq[1] = u.y; vq[2] = u.z; vq[3] = u.w;
-            } else {
-                vq[0] = vq[1] = vq[2] = vq[3] = 0.0f;
-            }
-        } else {
+    if (!(p.sum > 0.0)) { answer(stop, -1); return; }        // no distribution
+    c.ratio = c.less && with_q ? p.sum / q.sum : 0.0;
+    c.top_p = p.top;
+    c.top_q = q.top;
+    if (rank == 0 && tid == 0) a.cases[b] = c;
+    // ---- its sums, step by step; four steps of a warp at a time: their loads and exponentials overlap ----
+    const DraftRow row(a, b, d0, c);
+    double* sums = a.sums + (size_t)b * a.n_steps;
+    const int warps = blocks * DR_WARPS;
+    for (int s0 = rank * DR_WARPS + warp; s0 < a.n_steps; s0 += DR_AHEAD * warps) {
+        float vp[DR_AHEAD][4], vq[DR_AHEAD][4];
+        double part[DR_AHEAD];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                vp[e] = i0 + e < a.vocab ? lp[i0 + e] : -INFINITY;
-                vq[e] = i0 + e < a.vocab && less && with_q ? lq[i0 + e] : 0.0f;
-            }
+        for (int k = 0; k < DR_AHEAD; ++k) {
+            const int s = s0 + k * warps;
+            row.template load<VEC>(s < a.n_steps ? s * DR_STEP + 4 * lane : 0x7ffffff0, vp[k], vq[k]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = i0 + e < a.vocab ? left(i0 + e, vp[e], vq[e]) : 0.0;
-    };
-    cluster.sync();                                          // every block runs before another writes to it
-    const int me = rank * DR_WARPS + warp, from = me * each;
-    for (int round = 0; ; ++round) {
-        double sum = 0.0;
-        int s0 = 0;
-        // four steps at a time where they lie inside the vocabulary: their loads and sums overlap
-        if (VEC && wide == 1)
-            for (; s0 + 4 <= n_steps && from + (s0 + 4) * 128 <= a.vocab; s0 += 4) {
-                float4 vp[4], vq[4];
-                double part[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int i0 = from + (s0 + k) * 128 + 4 * lane;
-                    vp[k] = *reinterpret_cast<const float4*>(lp + i0);
-                    vq[k] = less && with_q ? *reinterpret_cast<const float4*>(lq + i0) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int i0 = from + (s0 + k) * 128 + 4 * lane;
-                    part[k] = (left(i0, vp[k].x, vq[k].x) + left(i0 + 1, vp[k].y, vq[k].y)) +
-                              (left(i0 + 2, vp[k].z, vq[k].z) + left(i0 + 3, vp[k].w, vq[k].w));
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) part[k] += __shfl_xor_sync(0xffffffffu, part[k], o);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (lane == 0) steps_s[warp][s0 + k] = part[k];
-                    sum += part[k];
-                }
-            }
-        for (int s = s0; s < n_steps; ++s) {
-            double part = 0.0;
-            for (int k = 0; k < wide; ++k) {
-                const int i0 = from + s * step + k * 128;
-                double w[4] = {0.0, 0.0, 0.0, 0.0};
-                if (i0 < a.vocab) four(i0 + 4 * lane, w);
-                part += (w[0] + w[1]) + (w[2] + w[3]);
-            }
-            part = warp_sum_d(part);
-            if (lane == 0) steps_s[warp][s] = part;
-            sum += part;
+        for (int k = 0; k < DR_AHEAD; ++k) {
+            const int i0 = (s0 + k * warps) * DR_STEP + 4 * lane;
+            part[k] = 0.0;
+            if (s0 + k * warps < a.n_steps)                  // (uniform over the warp)
+                part[k] = row.weight(i0, vp[k], vq[k], table_s);
         }
-        if (lane < blocks) *cluster.map_shared_rank(&sums_s[round][me], lane) = sum;
-        cluster.sync();                                      // every block has every sum
-        if (sum_of_stretches(sums_s[round]) > 0.0 || !less) break;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < DR_AHEAD; ++k) part[k] += __shfl_xor_sync(0xffffffffu, part[k], o);
+#pragma unroll
+        for (int k = 0; k < DR_AHEAD; ++k)
+            if (lane == 0 && s0 + k * warps < a.n_steps) sums[s0 + k * warps] = part[k];
+    }
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(DR_PICK) draft_pick_kernel(DraftArgs a) {
+    __shared__ double table_s[DR_TABLE];
+    __shared__ double ends_s[DR_PICK / 32];                  // the warps' sums
+    draft_table(table_s);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
+    pdl_prologue();
+    DraftCase c = a.cases[b];
+    if (c.stop < 0) return;
+    const int d0 = a.cu[b];
+    double* sums = a.sums + (size_t)b * a.n_steps;
+    const double u = (double)a.draw_u[b];
+    // a warp takes a stretch of whole chunks of 128 steps
+    const int chunks = (a.n_steps + 127) / 128, each = (chunks + DR_PICK / 32 - 1) / (DR_PICK / 32) * 128;
+    const int from = warp * each, to = min(a.n_steps, from + each);
+    for (;;) {
+        double mine = 0.0;
+        for (int s = from + lane; s < to; s += 32) mine += sums[s];
+        mine = warp_sum_d(mine);
+        if (lane == 0) ends_s[warp] = mine;
+        __syncthreads();
+        double total = 0.0;
+#pragma unroll
+        for (int w = 0; w < DR_PICK / 32; ++w) total += ends_s[w];
+        if (total > 0.0 || !c.less) break;                   // (uniform over the block)
         // nothing is left of p (rounding, or a number of 1 or more): from p itself
-        less = false;
+        c.less = 0;
+        const DraftRow row(a, b, d0, c);
+        for (int s = warp; s < a.n_steps; s += DR_PICK / 32) {
+            float vp[4], vq[4];
+            row.template load<VEC>(s * DR_STEP + 4 * lane, vp, vq);
+            const double part = warp_sum_d(row.weight(s * DR_STEP + 4 * lane, vp, vq, table_s));
+            if (lane == 0) sums[s] = part;
+        }
+        __syncthreads();
     }
-    // ---- the block whose stretch it is finds the token ----
-    if (warp == 0) {
-        const double* sums = sums_s[stop < n && !less ? 1 : 0];
-        const double want = (double)a.draw_u[b] * sum_of_stretches(sums);
-        // the stretch: the first whose end lies beyond `want`, else the last that holds anything
-        double w[4], run = 0.0;
+    if (warp != 0) return;
+    // the warp's stretch, then its chunk, then the step, then the token: each the first whose end lies beyond
+    // `want`, else the last that holds anything
+    double w[4], run = 0.0, want = 0.0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = sums[4 * lane + e];
-        const Crossing s = find_crossing(w, want, &run);
-        const int pick = max(0, s.first >= 0 ? s.first : s.last);
-        if (pick / DR_WARPS != rank) return;
-        // the step of it, the same way, and the token of the step
-        run = s.first >= 0 ? s.before_first : s.before_last;
-        const double* parts = steps_s[pick % DR_WARPS];
+    for (int e = 0; e < 4; ++e) {
+        w[e] = 4 * lane + e < DR_PICK / 32 ? ends_s[(4 * lane + e) % (DR_PICK / 32)] : 0.0;
+        want += w[e];
+    }
+    want = u * warp_sum_d(want);
+    const Crossing t = find_crossing(w, want, &run);
+    const int at = max(0, t.first >= 0 ? t.first : t.last);
+    run = t.first >= 0 ? t.before_first : t.before_last;
+    int step = -1, last_step = 0;
+    double before = 0.0, before_last = 0.0;
+    for (int s0 = at * each; s0 < min(a.n_steps, (at + 1) * each) && step < 0; s0 += 128) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = 4 * lane + e < n_steps ? parts[4 * lane + e] : 0.0;
-        const Crossing t = find_crossing(w, want, &run);
-        const int in = max(0, t.first >= 0 ? t.first : t.last);
-        run = t.first >= 0 ? t.before_first : t.before_last;
-        int token = -1, last = -1;
-        for (int k = 0; k < wide && token < 0; ++k) {
-            const int i0 = pick * each + in * step + k * 128;
-            four(i0 + 4 * lane, w);
-            const Crossing c = find_crossing(w, want, &run);
-            if (c.first >= 0) token = i0 + c.first;
-            if (c.last >= 0) last = i0 + c.last;
-        }
-        if (lane == 0) {
-            a.accepted[b] = stop;
-            a.tokens[b] = token >= 0 ? token : last;
-        }
+        for (int e = 0; e < 4; ++e) w[e] = s0 + 4 * lane + e < a.n_steps ? sums[s0 + 4 * lane + e] : 0.0;
+        const Crossing k = find_crossing(w, want, &run);
+        if (k.first >= 0) { step = s0 + k.first; before = k.before_first; }
+        if (k.last >= 0) { last_step = s0 + k.last; before_last = k.before_last; }
+    }
+    if (step < 0) { step = last_step; before = before_last; }
+    run = before;
+    const DraftRow row(a, b, d0, c);
+    float vp[4], vq[4];
+    row.template load<VEC>(step * DR_STEP + 4 * lane, vp, vq);
+    row.weights(step * DR_STEP + 4 * lane, vp, vq, table_s, w);
+    const Crossing k = find_crossing(w, want, &run);
+    if (lane == 0) {
+        a.accepted[b] = c.stop;
+        a.tokens[b] = step * DR_STEP + (k.first >= 0 ? k.first : k.last);
     }
 }
 
@@ -478,50 +521,50 @@ template <bool VEC> static int drafts_launch(const DraftArgs& a, int rows, cudaS
     if (a.draft_logits != nullptr) mf_launch(draft_pieces_kernel<VEC, true>, grid, dim3(DR_THREADS), 0, stream, a);
     else mf_launch(draft_pieces_kernel<VEC, false>, grid, dim3(DR_THREADS), 0, stream, a);
     if (int e = MF_LAUNCH_CHECK()) return e;
-    // as many blocks a sequence as the GPU holds at once: one an SM if that is the most a cluster takes, else two.
-    // us, one / two an SM, both launches: 1 sequence of 4 drafts with their logits 21.4 / 23.3, 8 of 4 36.0 / 45.8, 64 of
-    // 4 153 / 142, 64 of 0 to 7 looked up 78 / 70.
-    int blocks = DR_CLUSTER;
-    const bool few = (long long)a.n_seqs * blocks <= mf_sm_count();
-    while (blocks > 1 && (long long)a.n_seqs * blocks > 2 * mf_sm_count()) blocks >>= 1;
-    if (a.greedy) blocks = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.n_seqs * blocks);
-    cfg.blockDim = dim3(DR_WARPS * 32);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = blocks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = mf_pdl_enabled() ? 2 : 1;
-    if (few) cudaLaunchKernelEx(&cfg, draft_resolve_kernel<VEC, 1>, a, blocks);
-    else cudaLaunchKernelEx(&cfg, draft_resolve_kernel<VEC, 2>, a, blocks);
+    // what the GPU holds at once, and at least a step a warp
+    int blocks = 1;
+    if (!a.greedy) {
+        blocks = min(DR_MOST, DR_HELD * mf_sm_count() / a.n_seqs);
+        blocks = max(1, min(blocks, a.n_steps / DR_WARPS));
+    }
+    mf_launch(draft_sums_kernel<VEC>, dim3(a.n_seqs * blocks), dim3(DR_WARPS * 32), 0, stream, a, blocks);
+    if (int e = MF_LAUNCH_CHECK()) return e;
+    if (a.greedy) return 0;
+    mf_launch(draft_pick_kernel<VEC>, dim3(a.n_seqs), dim3(DR_PICK), 0, stream, a);
     return MF_LAUNCH_CHECK();
 }
 
-// pieces a row of `vocab` logits is read in (the scratch holds 16 bytes for each)
-extern "C" int mf_draft_pieces(int vocab) { return (vocab + DR_PIECE - 1) / DR_PIECE; }
+static int draft_pieces(int vocab) { return (vocab + DR_PIECE - 1) / DR_PIECE; }
+static int draft_steps_of(int vocab) { return (vocab + DR_STEP - 1) / DR_STEP; }
+// The scratch of a call in bytes (16-byte aligned): `rows` of logits in all, drafts' among them.
+extern "C" long long mf_draft_scratch(long long rows, int n_seqs, int vocab) {
+    return rows * draft_pieces(vocab) * (long long)sizeof(double2) + (long long)n_seqs * (long long)sizeof(DraftCase) +
+           (long long)n_seqs * draft_steps_of(vocab) * (long long)sizeof(double);
+}
 
 extern "C" int mf_verify_drafts(const float* logits, long long stride, const int* drafts, const int* cu,
                                 const float* draft_logits, long long draft_stride, const float* accept_u,
-                                const float* draw_u, double temperature, int* accepted, int* tokens, void* pieces,
+                                const float* draw_u, double temperature, int* accepted, int* tokens, void* scratch,
                                 int n_drafts, int n_seqs, int vocab, cudaStream_t stream) {
     if (n_seqs <= 0) return 0;
-    if (vocab <= 0 || n_drafts < 0 || !(temperature >= 0.0)) return MF_ERR_ARGUMENT;
+    if (vocab <= 0 || n_drafts < 0 || !(temperature >= 0.0 && temperature <= 1e30)) return MF_ERR_ARGUMENT;
     DraftArgs a{};
     a.logits = logits; a.stride = stride; a.drafts = drafts; a.cu = cu; a.draft_stride = draft_stride;
-    a.accept_u = accept_u; a.draw_u = draw_u; a.accepted = accepted; a.tokens = tokens; a.pieces = (double2*)pieces;
-    a.n_drafts = n_drafts; a.n_seqs = n_seqs; a.vocab = vocab; a.n_pieces = mf_draft_pieces(vocab);
+    a.accept_u = accept_u; a.draw_u = draw_u; a.accepted = accepted; a.tokens = tokens;
+    a.n_drafts = n_drafts; a.n_seqs = n_seqs; a.vocab = vocab; a.n_pieces = draft_pieces(vocab);
     a.greedy = temperature < 1e-6;
     a.draft_logits = a.greedy || n_drafts == 0 ? nullptr : draft_logits;
-    const double inv = a.greedy ? 0.0 : 1.0 / temperature;
-    a.inv_hi = (float)inv;
-    a.inv_lo = (float)(inv - (double)a.inv_hi);
+    a.base2 = a.greedy ? 0.0 : 1.4426950408889634074 / temperature;
+    a.base2_hi = (float)a.base2;
+    a.base2_lo = (float)(a.base2 - (double)a.base2_hi);
     a.temperature = (float)temperature;
     const long long rows = (long long)n_drafts + n_seqs + (a.draft_logits ? n_drafts : 0);
-    if (rows * a.n_pieces > 0x7fffffffLL || (long long)n_seqs * DR_CLUSTER > 0x7fffffffLL) return MF_ERR_UNSUPPORTED;
+    if (rows * a.n_pieces > 0x7fffffffLL || vocab > 0x7fffff00) return MF_ERR_UNSUPPORTED;
+    if (((uintptr_t)scratch & 15) || scratch == nullptr) return MF_ERR_ARGUMENT;
+    a.n_steps = draft_steps_of(vocab);
+    a.pieces = (double2*)scratch;
+    a.cases = (DraftCase*)(a.pieces + rows * a.n_pieces);
+    a.sums = (double*)(a.cases + n_seqs);
     const bool vec = vocab % 4 == 0 && stride % 4 == 0 && ((uintptr_t)logits & 15) == 0 &&
                      (a.draft_logits == nullptr || (draft_stride % 4 == 0 && ((uintptr_t)draft_logits & 15) == 0));
     return vec ? drafts_launch<true>(a, (int)rows, stream) : drafts_launch<false>(a, (int)rows, stream);

@@ -407,7 +407,8 @@ def _sig_attention_q8(lib: ctypes.CDLL) -> None:
 
 
 def _sig_drafts(lib: ctypes.CDLL) -> None:
-    lib.mf_draft_pieces.argtypes = [c_int]
+    lib.mf_draft_scratch.argtypes = [c_longlong, c_int, c_int]
+    lib.mf_draft_scratch.restype = c_longlong
     lib.mf_verify_drafts.argtypes = [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_void_p,
                                      c_void_p, ctypes.c_double, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                                      c_void_p]
@@ -2626,19 +2627,19 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.T
                           f"not {logits.shape[0]}")
     if cu_drafts.numel() != rows + 1 or accept_u.numel() != n or accepted.numel() != rows or tokens.numel() != rows:
         raise KernelError(f"{what}: sizes do not fit {n} drafts of {rows} sequences")
-    if not (math.isfinite(temperature) and temperature >= 0.0):
-        raise KernelError(f"{what}: temperature must be finite and not negative")
+    if not 0.0 <= temperature <= 1e30:
+        raise KernelError(f"{what}: temperature must lie between 0 and 1e30, not {temperature}")
     at, f32, i32 = _here(logits, what), torch.float32, torch.int32
     if draft_logits is not None and draft_logits.get_device() != at:
         raise KernelError(f"{what}: the drafts' logits must live on cuda:{at}")
     if rows == 0:
         return
-    # two numbers for every piece of a row
-    pieces = torch.empty(2 * (logits.shape[0] + (n if draft_logits is not None else 0)) *
-                         _fn("drafts", "mf_draft_pieces")(vocab), dtype=torch.float64, device=logits.device)
+    all_rows = logits.shape[0] + (n if draft_logits is not None else 0)
+    scratch = torch.empty(_fn("drafts", "mf_draft_scratch")(all_rows, rows, vocab), dtype=torch.uint8,
+                          device=logits.device)
     _check(_fn("drafts", "mf_verify_drafts")(
         logits.data_ptr(), logits.stride(0), _at(drafts, i32, at, "drafts"), _at(cu_drafts, i32, at, "cu_drafts"),
         None if draft_logits is None else draft_logits.data_ptr(),
         0 if draft_logits is None else draft_logits.stride(0), _at(accept_u, f32, at, "accept_u"),
         _at(draw_u, f32, at, "draw_u"), temperature, _at(accepted, i32, at, "accepted"), _at(tokens, i32, at, "tokens"),
-        pieces.data_ptr(), n, rows, vocab, _stream_of(at)), what, 2)
+        scratch.data_ptr(), n, rows, vocab, _stream_of(at)), what, 2 if temperature < 1e-6 else 3)

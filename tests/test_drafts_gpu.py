@@ -46,6 +46,23 @@ def test_against_the_plain_form(vocab, counts, with_logits, temperature):
     assert got == plain.verify(logits, drafts, cu, dl if with_logits else None, u, r, temperature)
 
 
+@pytest.mark.parametrize("with_logits", [True, False])
+def test_a_vocabulary_of_many_pieces(with_logits):
+    logits, drafts, cu, dl, u, r = make(300007, [2, 0, 5], 3)
+    got = run(logits, drafts, cu, dl if with_logits else None, u, r, 1.0)
+    assert got == plain.verify(logits, drafts, cu, dl if with_logits else None, u, r, 1.0)
+
+
+@pytest.mark.parametrize("temperature", [2e-6, 1e30])
+@pytest.mark.parametrize("with_logits", [True, False])
+def test_extreme_temperatures(temperature, with_logits):
+    logits, drafts, cu, dl, u, r = make(5000, [3, 3, 0], 3)
+    logits[:, 7::3] = -np.inf
+    logits[:, 6] = np.finfo(np.float32).min
+    got = run(logits, drafts, cu, dl if with_logits else None, u, r, temperature)
+    assert got == plain.verify(logits, drafts, cu, dl if with_logits else None, u, r, temperature)
+
+
 @pytest.mark.parametrize("vocab", [389, 20000])
 def test_the_same_distribution_is_always_accepted_and_another_never(vocab):
     logits, drafts, cu, _, u, r = make(vocab, [3, 5], 2)

@@ -120,6 +120,7 @@ def test_read_refuses(change, why):
     (dict(tokens=torch.zeros(3, dtype=I32)), "sizes"),
     (dict(temperature=-0.1), "temperature"),
     (dict(temperature=float("inf")), "temperature"),
+    (dict(temperature=2e30), "temperature"),
     (dict(temperature=float("nan")), "temperature"),
 ])
 def test_verify_refuses(change, why):
