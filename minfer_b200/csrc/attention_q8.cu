@@ -28,6 +28,7 @@ struct AttnQ8Args {
     void* out;                     // [tokens][n_heads][hd]
     float* partial;                // scratch, see the kernels
     int n_tokens, n_rows, n_heads, n_kv, hd, window;
+    int max_end;                   // positions that the page table has room for
     int n_splits;                  // parts that a row's pages are shared out to
     int q_groups;                  // blocks along the longest row's matrix rows
     float scale;
@@ -129,12 +130,18 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {          // an 8 x 
 struct AqRow {
     int tok0, count, end, base0, pages, items;
 };
+// A row's tokens and its end, brought inside what there is (numbers that the device gave may be anything; an end
+// behind the page table is reported, and tokens in front of position 0 see nothing).
+__device__ __forceinline__ void aq_bounds(const AttnQ8Args& a, int b, int* tok0, int* count, int* end) {
+    const int from = a.cu_seqlens[b], to = a.cu_seqlens[b + 1], e = a.seq_end[b];
+    *tok0 = from;
+    *count = from >= 0 && from <= to && to <= a.n_tokens ? to - from : 0;
+    *end = min(max(e, 0), a.max_end);
+    if (e > a.max_end && *count > 0 && threadIdx.x == 0) atomicOr(a.status, MF_STATUS_BAD_POSITION);
+}
 __device__ __forceinline__ AqRow aq_row(const AttnQ8Args& a, int b, int rows_a_block) {
     AqRow r;
-    r.tok0 = a.cu_seqlens[b];
-    r.count = a.cu_seqlens[b + 1] - r.tok0;
-    r.end = a.seq_end[b];
-    if (r.count <= 0 || r.tok0 < 0 || r.tok0 + r.count > a.n_tokens) r.count = 0;
+    aq_bounds(a, b, &r.tok0, &r.count, &r.end);
     const int first = r.end - r.count;
     r.base0 = (a.window > 0 ? max(0, first - a.window + 1) : 0) & ~(MF_PAGE - 1);
     r.items = a.n_kv * min(a.q_groups, (r.count * (a.n_heads / a.n_kv) + rows_a_block - 1) / rows_a_block);
@@ -798,9 +805,10 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, hk = blockIdx.y / a.q_groups, qg = blockIdx.y - hk * a.q_groups, b = blockIdx.z;
     const int G = a.n_heads / a.n_kv;
-    const int tok0 = a.cu_seqlens[b], count = a.cu_seqlens[b + 1] - tok0, end = a.seq_end[b];
+    int tok0, count, end;
+    aq_bounds(a, b, &tok0, &count, &end);
     const int r0 = qg * AG_ROWS, rows = min(AG_ROWS, count * G - r0);
-    if (rows <= 0 || tok0 < 0 || tok0 + count > a.n_tokens) { pdl_wait(); return; }
+    if (rows <= 0) { pdl_wait(); return; }
     const int first = end - count + r0 / G, last = end - count + (r0 + rows - 1) / G;
     const int lo_all = a.window > 0 ? max(0, first - a.window + 1) : 0;
     const int base0 = lo_all & ~(MF_PAGE - 1), pages = max(0, (last - base0 + MF_PAGE) / MF_PAGE);
@@ -935,16 +943,22 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
 // the unnormalised output; a split without a visible key has a maximum of -infinity and no output.
 // ------------------------------------------------------------------------------------------
 template <typename T>
-__global__ void attention_q8_merge_kernel(const float* partial, T* __restrict__ out, int n_splits, int hd, int n_heads,
-                                          const int* cu_seqlens, int n_rows) {
+__global__ void attention_q8_merge_kernel(AttnQ8Args a) {
     pdl_prologue();
+    const int n_splits = a.n_splits, hd = a.hd, G = a.n_heads / a.n_kv;
     extern __shared__ float mq_s[];                        // [n_splits] factors
     __shared__ float red_s[33];
     const size_t th = blockIdx.x;
-    // tokens of no row stay as they are
-    const int token = blockIdx.x / n_heads;
-    if (token < cu_seqlens[0] || token >= cu_seqlens[n_rows]) return;
-    const float* p = partial + th * n_splits * (hd + 2);
+    // tokens that no row has brought stay as they are
+    const int token = blockIdx.x / a.n_heads, head = blockIdx.x - token * a.n_heads;
+    bool held = false;
+    for (int b = threadIdx.x; b < a.n_rows; b += blockDim.x) {
+        const int from = a.cu_seqlens[b], to = a.cu_seqlens[b + 1];
+        if (from >= 0 && from <= token && token < to && to <= a.n_tokens)
+            held |= (long long)(token - from) * G + head % G < (long long)a.q_groups * AG_ROWS;
+    }
+    if (!__syncthreads_or(held)) return;
+    const float* p = a.partial + th * n_splits * (hd + 2);
     float m = AQ_NEG;
     for (int s = threadIdx.x; s < n_splits; s += blockDim.x) m = fmaxf(m, p[(size_t)s * (hd + 2)]);
     m = block_max(m, red_s);
@@ -965,7 +979,7 @@ __global__ void attention_q8_merge_kernel(const float* partial, T* __restrict__ 
             const float f = mq_s[s];
             if (f != -1.0f) o = fmaf(p[(size_t)s * (hd + 2) + 2 + d], f, o);
         }
-        out[th * hd + d] = from_f32<T>(o * inv);
+        ((T*)a.out)[th * hd + d] = from_f32<T>(o * inv);
     }
 }
 
@@ -1110,9 +1124,10 @@ extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v
     if (hd % 16 != 0 || hd < 16 || hd > 256 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv != 0) return MF_ERR_UNSUPPORTED;
     if ((dtype != MF_DTYPE_F32 && dtype != MF_DTYPE_BF16) || (fmt != MF_Q8_E4M3 && fmt != MF_Q8_INT8))
         return MF_ERR_UNSUPPORTED;
+    if (table_stride > (1 << 24)) return MF_ERR_UNSUPPORTED;         // (positions are 32 bits, with room to add)
     if (table_stride <= 0 || n_pages <= 0 || ring < 0 || ring % MF_PAGE != 0 || window < 0 || status == nullptr)
         return MF_ERR_ARGUMENT;
-    const AqPlan plan = aq_plan(n_tokens, n_rows, max_row_tokens, span, n_heads, n_kv, hd, dtype);
+    AqPlan plan = aq_plan(n_tokens, n_rows, max_row_tokens, span, n_heads, n_kv, hd, dtype);
     if (plan.floats > 0 && (partial == nullptr || ((uintptr_t)partial & 15))) return MF_ERR_ARGUMENT;
     if (ring > 0 && (window <= 0 || max_row_tokens > ring - window + 1)) return MF_ERR_ARGUMENT;
     if (n_rows > 65535) return MF_ERR_UNSUPPORTED;
@@ -1128,6 +1143,10 @@ extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v
     const long long groups = ((long long)max_row_tokens * (n_heads / n_kv) + plan.rows - 1) / plan.rows;
     if (groups * n_kv > 32767) return MF_ERR_UNSUPPORTED;
     a.q_groups = (int)groups;
+    a.max_end = ring > 0 ? 1 << 30 : table_stride * MF_PAGE;
+    // (the pages of all items are counted in 32 bits)
+    const long long row_pages = ring > 0 ? ((long long)window + n_tokens) / MF_PAGE + 3 : table_stride;
+    if (plan.splits < 0 && row_pages * groups * n_kv * n_rows > 0x7fffffffLL) plan.splits = 1;
     const int items = (int)(groups * n_kv), n_splits = a.n_splits;
     const dim3 grid(n_splits, items, n_rows);
     int e;
@@ -1151,9 +1170,9 @@ extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v
     if ((long long)n_tokens * n_heads > 0x7fffffffLL) return MF_ERR_UNSUPPORTED;
     if (dtype == MF_DTYPE_F32)
         mf_launch(attention_q8_merge_kernel<float>, dim3((unsigned)(n_tokens * n_heads)), dim3(threads),
-                  (size_t)n_splits * 4, stream, partial, (float*)out, n_splits, hd, n_heads, cu_seqlens, n_rows);
+                  (size_t)n_splits * 4, stream, a);
     else
         mf_launch(attention_q8_merge_kernel<__nv_bfloat16>, dim3((unsigned)(n_tokens * n_heads)), dim3(threads),
-                  (size_t)n_splits * 4, stream, partial, (__nv_bfloat16*)out, n_splits, hd, n_heads, cu_seqlens, n_rows);
+                  (size_t)n_splits * 4, stream, a);
     return MF_LAUNCH_CHECK();
 }

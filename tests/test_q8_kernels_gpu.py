@@ -251,6 +251,37 @@ def test_a_page_that_is_not_there_is_not_read(dtype, dim):
     assert int(st.item()) == 2 and torch.equal(got[1], clean[1])
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+@pytest.mark.parametrize("longest", [200, 4000, 40000])
+@pytest.mark.parametrize("window", [0, 70])
+def test_lengths_and_offsets_that_are_anything(longest, window, dtype, dim):
+    """What the device gives as lengths and offsets is brought inside the page table and the tokens."""
+    heads, kv, fmt, big = 4, 2, torch.int8, 2 ** 31 - 1
+    gen, rng = torch.Generator().manual_seed(1), np.random.RandomState(2)
+    ends = [longest, 90, 80, 150, 33, 20]
+    table, n_pages = make_table(ends, 0, rng)
+    pages = make_pages(table, n_pages, ends, 0, kv, dim, fmt, gen)
+    q = torch.randn(6, heads, dim, generator=gen).to(dtype).to(DEV)
+    cu = [0, 1, 2, 3, 4, 5, 6]
+    want, *sizes = plain.attention(q, pages, cu, ends, table, 0, heads, kv, window, 0.2)
+    tol = plain.attention_tolerance(want, *sizes, dtype, dim, fmt)
+
+    def call(cu, ends):
+        out, st = torch.full_like(q, 7.0), status_word()
+        K.attention_paged_q8(q, pages, ints(cu), ints(ends), ints(table), len(table[0]), 0, out, 1, longest, heads, kv,
+                             dim, window, 0.2, st)
+        return out, (out.double().cpu() - want).abs() <= tol, int(st.item())
+    for wild in (big, big - 31, 2 ** 30, 64 * len(table[0]) + 1):
+        out, right, st = call(cu, [ends[0], wild, ends[2], wild, ends[4], ends[5]])
+        assert st == 2 and right[[0, 2, 4, 5]].all()
+    for wild in (-1, -2 ** 31, -2 ** 31 + 40):
+        out, right, st = call(cu, [ends[0], wild, ends[2], wild, ends[4], ends[5]])
+        assert st == 0 and right[[0, 2, 4, 5]].all() and (out[[1, 3]] == 0).all()
+    for wild in (-1, -2 ** 31, 7, big):
+        out, right, st = call([0, 1, wild, 3, 4, 5, 6], ends)
+        assert st == 0 and right[[0, 3, 4, 5]].all() and (out[1:3] == 7.0).all()
+
+
 @pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float32, 64)])
 def test_offsets_beyond_32_bits(dtype, dim):
     heads, kv, fmt = 8, 8, torch.int8
