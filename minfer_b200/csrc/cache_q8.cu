@@ -289,8 +289,8 @@ extern "C" int mf_rope_kvstore_q8(const float* qkv, int n_partials, const float*
 
 // ------------------------------------------------------------------------------------------
 // Pages read back: out [rows * out_stride][n_kv][64][hd] in bfloat16 or float32, a row's pages in the order
-// of the page table; places that hold no position of the row are zeros, and so are pages behind the
-// table's.
+// of the page table, as many as the output has; places that hold no position of the row are zeros, and so are
+// pages behind the table's.
 //
 // Bound by bytes: 1 read and 2 (4) written an element.  A block takes one page of one key/value
 // head, K or V: a thread's unit is 8 codes, so that a warp's stores are whole lines without gaps (16 codes,
@@ -342,9 +342,9 @@ __global__ void __launch_bounds__(RD_THREADS) read_pages_q8_kernel(ReadQ8Args a)
     const int page = index < a.table_stride ? a.page_table[(long long)row * a.table_stride + index] : -1;
     // places [0, n) of the page hold positions of the row (a ring that is full: all of them; the ring's
     // lap does not matter to what a place holds)
-    const int span = min(a.ring > 0 ? min(end, a.ring) : end, a.table_stride * MF_PAGE);
+    const int span = min(a.ring > 0 ? min(end, a.ring) : end, min(a.table_stride, a.out_stride) * MF_PAGE);
     int n = min(MF_PAGE, span - index * MF_PAGE);
-    // (a length beyond the table)
+    // (a length beyond the table, or the output)
     if (a.ring == 0 && end > span && index == 0 && hk == 0 && threadIdx.x == 0) atomicOr(a.status, MF_STATUS_BAD_POSITION);
     if (n <= 0 && !a.fill) { pdl_wait(); return; }
     const bool there = page >= 0 && page < a.n_pages;
@@ -406,9 +406,9 @@ extern "C" int mf_read_pages_q8(const void* k_codes, const void* v_codes, const 
                                 int fmt, int fill, int for_attention, unsigned* status, cudaStream_t stream) {
     if (rows <= 0) return 0;
     if (hd % 16 != 0 || hd < 16 || hd > 256 || n_kv <= 0 || n_kv > 65535) return MF_ERR_UNSUPPORTED;
-    if (ring < 0 || ring % MF_PAGE != 0 || table_stride <= 0 || out_stride < table_stride || n_pages <= 0)
+    if (ring < 0 || ring % MF_PAGE != 0 || table_stride <= 0 || out_stride <= 0 || n_pages <= 0)
         return MF_ERR_ARGUMENT;
-    if ((long long)rows * out_stride > 0x7fffffffLL || table_stride > 0x7fffffff / MF_PAGE) return MF_ERR_UNSUPPORTED;
+    if ((long long)rows * out_stride > 0x7fffffffLL || table_stride > 0x7fffffff / MF_PAGE || out_stride > 0x7fffffff / MF_PAGE) return MF_ERR_UNSUPPORTED;
     if (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return MF_ERR_UNSUPPORTED;
     if ((dtype != MF_DTYPE_F32 && dtype != MF_DTYPE_BF16) || (fmt != MF_Q8_E4M3 && fmt != MF_Q8_INT8))
         return MF_ERR_UNSUPPORTED;

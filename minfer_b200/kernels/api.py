@@ -1257,7 +1257,7 @@ def read_pages_q8(pages: Q8Pages, page_table: torch.Tensor, table_stride: int, r
 def _read_pages_q8(pages: Q8Pages, fmt: int, page_table: torch.Tensor, table_stride: int, out_stride: int, ring: int,
                    seq_end: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, status: torch.Tensor, fill: bool,
                    for_attention: bool) -> None:
-    """``out_stride`` pages a row in the output (behind the table's: zeros).  ``for_attention``: a position whose
+    """``out_stride`` pages a row in the output: the table's first ones (behind the table's: zeros).  ``for_attention``: a position whose
     key or value is NaN becomes a key of NaN with a value of zeros."""
     at, f32, i32, codes, dt = k_out.get_device(), torch.float32, torch.int32, pages.k.dtype, k_out.dtype
     _check(_fn("cache_q8", "mf_read_pages_q8")(
@@ -1345,9 +1345,12 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
         span = min(span, window + max_row_tokens + PAGE - 1)
     if max_row_tokens >= 32 and dt is torch.bfloat16 and head_dim in (64, 128) and q8_reads_back(
             tokens, rows, max_row_tokens, span, n_heads, n_kv, head_dim, sm_count(q.device)):
-        # pages of the rows read back, as many rows at a time as the scratch takes; a tile of the kernel is
-        # two pages, so a row has an even number of them (the last one zeros where there is none)
-        wide = table_stride + (table_stride & 1)
+        # pages of the rows read back, as many of a row as its positions can lie in and as many rows at a time as
+        # the scratch takes; a tile of the kernel is two pages, so a row has an even number of them (the last one
+        # zeros where there is none)
+        _at(page_table, i32, at, "page_table")
+        wide = max(1, min(table_stride, -(-(min(max_end, ring) if ring else max_end) // PAGE)))
+        wide += wide & 1
         some = max(1, min(rows, Q8_PORTION_BYTES // (wide * n_kv * PAGE * head_dim * 4)))
         k = torch.empty((some * wide, n_kv, PAGE, head_dim), dtype=torch.bfloat16, device=q.device)
         v = torch.empty_like(k)

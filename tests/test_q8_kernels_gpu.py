@@ -307,6 +307,30 @@ def test_offsets_beyond_32_bits(dtype, dim):
     assert torch.equal(out[1][0].cpu(), (small[1][0][1].float() * small[1][1][1].unsqueeze(-1)).to(dtype))
 
 
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("back", [True, False])
+def test_a_page_table_wider_than_its_rows(window, back, monkeypatch):
+    """Places that no position of a row can lie in cost nothing and change nothing; a length beyond ``max_end``
+    is reported where that sizes what is read back."""
+    monkeypatch.setattr(K, "q8_reads_back", lambda *a: back)
+    heads, kv, dim, fmt = 6, 2, 128, torch.int8
+    gen, rng = torch.Generator().manual_seed(41), np.random.RandomState(6)
+    ends, cu = [140, 75, 33], [0, 40, 108, 141]
+    ring = 192 if window else 0
+    table, n_pages = make_table(ends, ring, rng)
+    pages = make_pages(table, n_pages, ends, ring, kv, dim, fmt, gen)
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(torch.bfloat16).to(DEV)
+    clean = run_attention(q, pages, cu, ends, table, ring, heads, kv, dim, window, 0.1)
+    wide = [r + [n_pages + 7] * 4000 for r in table]
+    before = torch.cuda.max_memory_allocated()
+    assert torch.equal(run_attention(q, pages, cu, ends, wide, ring, heads, kv, dim, window, 0.1), clean)
+    assert torch.cuda.max_memory_allocated() - before < 2 ** 24
+    if back and not window:
+        st = status_word()
+        run_attention(q, pages, cu, ends, table, ring, heads, kv, dim, window, 0.1, status=st, max_end=100)
+        assert int(st.item()) & 2
+
+
 def test_captured_twice_and_on_another_stream():
     heads, kv, dim, fmt = 28, 4, 128, torch.float8_e4m3fn
     gen, rng = torch.Generator().manual_seed(1), np.random.RandomState(2)
