@@ -288,19 +288,14 @@ extern "C" int mf_rope_kvstore_q8(const float* qkv, int n_partials, const float*
 }
 
 // ------------------------------------------------------------------------------------------
-// Pages read back: out [rows * out_stride][n_kv][64][hd] in bfloat16 or float32, a row's pages in the order
-// of the page table, as many as the output has; places that hold no position of the row are zeros, and so are
-// pages behind the table's.
+// Pages read back: out [rows * table_stride][n_kv][64][hd] in bfloat16 or float32, a row's pages in the order
+// of the page table; places that hold no position of the row are zeros.
 //
 // Bound by bytes: 1 read and 2 (4) written an element.  A block takes one page of one key/value
 // head, K or V: a thread's unit is 8 codes, so that a warp's stores are whole lines without gaps (16 codes,
 // two stores a thread: 72 us where this takes 62), and all of a thread's loads of a round are
 // issued before the first conversion.  4 sequences of 15,001 to 31,999 positions, 4 heads of 128, in a table
 // of 500 pages a row: 62.5 us = 5.8 TB/s of what is read and written, the zeros behind the shorter rows included.
-//
-// FOR_ATTENTION: what a kernel reads that multiplies masked probabilities (zeros) with values.  A value of
-// NaN would reach rows that do not see it; so a position whose key or value is NaN becomes a key of NaN
-// with a value of zeros: its score is NaN for those who see it, and masked for the others.
 // ------------------------------------------------------------------------------------------
 struct ReadQ8Args {
     const uint8_t* k_codes;
@@ -308,7 +303,7 @@ struct ReadQ8Args {
     const float* k_scales;
     const float* v_scales;
     const int* page_table;
-    int table_stride, out_stride, ring, n_pages;
+    int table_stride, ring, n_pages;
     const int* seq_end;
     void* k_out;
     void* v_out;
@@ -332,19 +327,19 @@ template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16*
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-template <typename T, int FMT, bool FOR_ATTENTION>
+template <typename T, int FMT>
 __global__ void __launch_bounds__(RD_THREADS) read_pages_q8_kernel(ReadQ8Args a) {
     pdl_launch_dependents();
     const int hk = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
-    const int row = blockIdx.x / a.out_stride, index = blockIdx.x - row * a.out_stride;
+    const int row = blockIdx.x / a.table_stride, index = blockIdx.x - row * a.table_stride;
     const int end = a.seq_end[row];
-    const int page = index < a.table_stride ? a.page_table[(long long)row * a.table_stride + index] : -1;
+    const int page = a.page_table[blockIdx.x];
     // places [0, n) of the page hold positions of the row (a ring that is full: all of them; the ring's
     // lap does not matter to what a place holds)
-    const int span = min(a.ring > 0 ? min(end, a.ring) : end, min(a.table_stride, a.out_stride) * MF_PAGE);
+    const int span = min(a.ring > 0 ? min(end, a.ring) : end, a.table_stride * MF_PAGE);
     int n = min(MF_PAGE, span - index * MF_PAGE);
-    // (a length beyond the table, or the output)
+    // (a length beyond the table)
     if (a.ring == 0 && end > span && index == 0 && hk == 0 && threadIdx.x == 0) atomicOr(a.status, MF_STATUS_BAD_POSITION);
     if (n <= 0 && !a.fill) { pdl_wait(); return; }
     const bool there = page >= 0 && page < a.n_pages;
@@ -358,7 +353,6 @@ __global__ void __launch_bounds__(RD_THREADS) read_pages_q8_kernel(ReadQ8Args a)
     const long long from = there ? ((long long)page * a.n_kv + hk) * MF_PAGE : 0;
     const uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + from * a.hd;
     const float* scales = (is_v ? a.v_scales : a.k_scales) + from;
-    const float* other = (is_v ? a.k_scales : a.v_scales) + from;
     T* out = (T*)(is_v ? a.v_out : a.k_out) + ((long long)blockIdx.x * a.n_kv + hk) * MF_PAGE * a.hd;
     for (int u0 = threadIdx.x; u0 < units; u0 += 4 * RD_THREADS) {
         uint2 w[4];
@@ -371,11 +365,6 @@ __global__ void __launch_bounds__(RD_THREADS) read_pages_q8_kernel(ReadQ8Args a)
             if (u < units && place < n) {
                 w[i] = *reinterpret_cast<const uint2*>(codes + (long long)u * 8);
                 s[i] = scales[place];
-                if (FOR_ATTENTION) {
-                    const float so = other[place];
-                    if (is_v && s[i] != s[i]) s[i] = 0.0f;
-                    else if (!is_v && so != so) s[i] = so;
-                }
             }
         }
 #pragma unroll
@@ -393,33 +382,32 @@ __global__ void __launch_bounds__(RD_THREADS) read_pages_q8_kernel(ReadQ8Args a)
     }
 }
 
-template <typename T, int FMT> static int read_launch(const ReadQ8Args& a, bool for_attention, cudaStream_t stream) {
-    const dim3 grid((unsigned)(a.rows * a.out_stride), a.n_kv, 2);
-    if (for_attention) mf_launch(read_pages_q8_kernel<T, FMT, true>, grid, dim3(RD_THREADS), 0, stream, a);
-    else mf_launch(read_pages_q8_kernel<T, FMT, false>, grid, dim3(RD_THREADS), 0, stream, a);
+template <typename T, int FMT> static int read_launch(const ReadQ8Args& a, cudaStream_t stream) {
+    const dim3 grid((unsigned)(a.rows * a.table_stride), a.n_kv, 2);
+    mf_launch(read_pages_q8_kernel<T, FMT>, grid, dim3(RD_THREADS), 0, stream, a);
     return MF_LAUNCH_CHECK();
 }
 
 extern "C" int mf_read_pages_q8(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales,
-                                const int* page_table, int table_stride, int out_stride, int ring, int n_pages,
+                                const int* page_table, int table_stride, int ring, int n_pages,
                                 const int* seq_end, void* k_out, void* v_out, int rows, int n_kv, int hd, int dtype,
-                                int fmt, int fill, int for_attention, unsigned* status, cudaStream_t stream) {
+                                int fmt, int fill, unsigned* status, cudaStream_t stream) {
     if (rows <= 0) return 0;
     if (hd % 16 != 0 || hd < 16 || hd > 256 || n_kv <= 0 || n_kv > 65535) return MF_ERR_UNSUPPORTED;
-    if (ring < 0 || ring % MF_PAGE != 0 || table_stride <= 0 || out_stride <= 0 || n_pages <= 0)
+    if (ring < 0 || ring % MF_PAGE != 0 || table_stride <= 0 || n_pages <= 0)
         return MF_ERR_ARGUMENT;
-    if ((long long)rows * out_stride > 0x7fffffffLL || table_stride > 0x7fffffff / MF_PAGE || out_stride > 0x7fffffff / MF_PAGE) return MF_ERR_UNSUPPORTED;
+    if ((long long)rows * table_stride > 0x7fffffffLL || table_stride > 0x7fffffff / MF_PAGE) return MF_ERR_UNSUPPORTED;
     if (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return MF_ERR_UNSUPPORTED;
     if ((dtype != MF_DTYPE_F32 && dtype != MF_DTYPE_BF16) || (fmt != MF_Q8_E4M3 && fmt != MF_Q8_INT8))
         return MF_ERR_UNSUPPORTED;
     ReadQ8Args a{};
     a.k_codes = (const uint8_t*)k_codes; a.v_codes = (const uint8_t*)v_codes; a.k_scales = k_scales;
-    a.v_scales = v_scales; a.page_table = page_table; a.table_stride = table_stride; a.out_stride = out_stride;
+    a.v_scales = v_scales; a.page_table = page_table; a.table_stride = table_stride;
     a.ring = ring; a.n_pages = n_pages; a.seq_end = seq_end; a.k_out = k_out; a.v_out = v_out; a.rows = rows;
     a.n_kv = n_kv; a.hd = hd; a.fill = fill; a.status = status;
     if (dtype == MF_DTYPE_F32)
-        return fmt == MF_Q8_E4M3 ? read_launch<float, MF_Q8_E4M3>(a, for_attention != 0, stream)
-                                 : read_launch<float, MF_Q8_INT8>(a, for_attention != 0, stream);
-    return fmt == MF_Q8_E4M3 ? read_launch<__nv_bfloat16, MF_Q8_E4M3>(a, for_attention != 0, stream)
-                             : read_launch<__nv_bfloat16, MF_Q8_INT8>(a, for_attention != 0, stream);
+        return fmt == MF_Q8_E4M3 ? read_launch<float, MF_Q8_E4M3>(a, stream)
+                                 : read_launch<float, MF_Q8_INT8>(a, stream);
+    return fmt == MF_Q8_E4M3 ? read_launch<__nv_bfloat16, MF_Q8_E4M3>(a, stream)
+                             : read_launch<__nv_bfloat16, MF_Q8_INT8>(a, stream);
 }

@@ -395,8 +395,15 @@ def _sig_moe(lib: ctypes.CDLL) -> None:
 def _sig_cache_q8(lib: ctypes.CDLL) -> None:
     lib.mf_rope_kvstore_q8.argtypes = ([c_void_p, c_int] + [c_void_p] * 13 + [c_int] * 11 +
                                        [c_void_p, c_void_p])
-    lib.mf_read_pages_q8.argtypes = ([c_void_p] * 5 + [c_int] * 4 + [c_void_p] * 3 + [c_int] * 7 +
+    lib.mf_read_pages_q8.argtypes = ([c_void_p] * 5 + [c_int] * 3 + [c_void_p] * 3 + [c_int] * 6 +
                                      [c_void_p, c_void_p])
+
+
+def _sig_attention_q8_tc(lib: ctypes.CDLL) -> None:
+    lib.mf_attention_q8_tc_scratch.argtypes = [c_int] * 6
+    lib.mf_attention_q8_tc_scratch.restype = c_longlong
+    lib.mf_attention_q8_tc.argtypes = ([c_void_p] * 8 + [c_int] * 3 + [c_void_p, c_void_p] + [c_int] * 8 + [c_float] +
+                                       [c_int] * 2 + [c_void_p, c_void_p])
 
 
 def _sig_attention_q8(lib: ctypes.CDLL) -> None:
@@ -414,7 +421,7 @@ def _sig_drafts(lib: ctypes.CDLL) -> None:
                                      c_void_p]
 
 
-_SIGNATURES = {"cache_q8": _sig_cache_q8, "attention_q8": _sig_attention_q8, "drafts": _sig_drafts,
+_SIGNATURES = {"cache_q8": _sig_cache_q8, "attention_q8": _sig_attention_q8, "attention_q8_tc": _sig_attention_q8_tc, "drafts": _sig_drafts,
                "retention": _sig_retention, "outer_scan": _sig_outer_scan, "delta_rule": _sig_delta_rule, "attention_talk": _sig_attention_talk, "moe": _sig_moe,
                "attention_prefill_tc": _sig_attention_prefill_tc, "recurrent": _sig_recurrent,
                "mixer_prep": _sig_mixer_prep,
@@ -1250,22 +1257,13 @@ def read_pages_q8(pages: Q8Pages, page_table: torch.Tensor, table_stride: int, r
     want = rows * table_stride * n_kv * PAGE * head_dim
     if k_out.dtype != v_out.dtype or k_out.numel() != want or v_out.numel() != want:
         raise KernelError(f"{what}: the outputs must be [rows * table_stride, {n_kv}, {PAGE}, {head_dim}] of one type")
-    _here(k_out, what)
-    _read_pages_q8(pages, fmt, page_table, table_stride, table_stride, ring, seq_end, k_out, v_out, status, fill, False)
-
-
-def _read_pages_q8(pages: Q8Pages, fmt: int, page_table: torch.Tensor, table_stride: int, out_stride: int, ring: int,
-                   seq_end: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, status: torch.Tensor, fill: bool,
-                   for_attention: bool) -> None:
-    """``out_stride`` pages a row in the output: the table's first ones (behind the table's: zeros).  ``for_attention``: a position whose
-    key or value is NaN becomes a key of NaN with a value of zeros."""
-    at, f32, i32, codes, dt = k_out.get_device(), torch.float32, torch.int32, pages.k.dtype, k_out.dtype
+    at, f32, i32, codes, dt = _here(k_out, what), torch.float32, torch.int32, pages.k.dtype, k_out.dtype
     _check(_fn("cache_q8", "mf_read_pages_q8")(
         _at(pages.k, codes, at, "keys"), _at(pages.v, codes, at, "values"), _at(pages.k_scale, f32, at, "key scales"),
-        _at(pages.v_scale, f32, at, "value scales"), _at(page_table, i32, at, "page_table"), table_stride, out_stride,
-        ring, pages.k.shape[0], _at(seq_end, i32, at, "seq_end"), _at(k_out, dt, at, "k_out"),
-        _at(v_out, dt, at, "v_out"), seq_end.numel(), pages.k.shape[1], pages.k.shape[3], dtype_code(dt), fmt,
-        1 if fill else 0, 1 if for_attention else 0, _at(status, i32, at, "status"), _stream_of(at)), "read_pages_q8")
+        _at(pages.v_scale, f32, at, "value scales"), _at(page_table, i32, at, "page_table"), table_stride, ring,
+        pages.k.shape[0], _at(seq_end, i32, at, "seq_end"), _at(k_out, dt, at, "k_out"), _at(v_out, dt, at, "v_out"),
+        rows, n_kv, head_dim, dtype_code(dt), fmt, 1 if fill else 0, _at(status, i32, at, "status"), _stream_of(at)),
+        what)
 
 
 _Q8_PLANS: Dict[tuple, tuple] = {}
@@ -1345,23 +1343,25 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
         span = min(span, window + max_row_tokens + PAGE - 1)
     if max_row_tokens >= 32 and dt is torch.bfloat16 and head_dim in (64, 128) and q8_reads_back(
             tokens, rows, max_row_tokens, span, n_heads, n_kv, head_dim, sm_count(q.device)):
-        # pages of the rows read back, as many of a row as its positions can lie in and as many rows at a time as
-        # the scratch takes; a tile of the kernel is two pages, so a row has an even number of them (the last one
-        # zeros where there is none)
-        _at(page_table, i32, at, "page_table")
-        wide = max(1, min(table_stride, -(-(min(max_end, ring) if ring else max_end) // PAGE)))
-        wide += wide & 1
-        some = max(1, min(rows, Q8_PORTION_BYTES // (wide * n_kv * PAGE * head_dim * 4)))
-        k = torch.empty((some * wide, n_kv, PAGE, head_dim), dtype=torch.bfloat16, device=q.device)
-        v = torch.empty_like(k)
-        places = torch.arange(some * wide, dtype=torch.int32, device=q.device)
+        # positions of a row in the scratch: what its tokens can see, in tiles of 128 from a tile's border on
+        reach = max(1, max_end)
+        if window > 0:
+            reach = min(reach, window + max_row_tokens + 126)
+        stretch = -(-reach // 128) * 128
+        some = max(1, min(rows, Q8_PORTION_BYTES // (stretch * n_kv * head_dim * 4)))
+        scratch = torch.empty(_fn("attention_q8_tc", "mf_attention_q8_tc_scratch")(
+            tokens, some, stretch, n_heads, n_kv, head_dim) + 1023, dtype=torch.uint8, device=q.device)
+        base, ends, offsets = scratch.data_ptr(), _at(seq_end, i32, at, "seq_end"), _at(cu_seqlens, i32, at, "cu_seqlens")
+        table = _at(page_table, i32, at, "page_table")
+        # (as many rows at a time as the scratch takes; its queries are those of all tokens)
         for first in range(0, rows, some):
-            last = min(rows, first + some)
-            ends = seq_end[first:last]
-            _read_pages_q8(pages, fmt, page_table.view(-1)[first * table_stride:], table_stride, wide, ring, ends, k, v,
-                           status, True, True)
-            attention_prefill_tc_paged(q, k, v, cu_seqlens[first:last + 1], ends, places, wide, ring, out, last - first,
-                                       int(max_row_tokens), n_heads, n_kv, head_dim, int(window), float(scale), status)
+            _check(_fn("attention_q8_tc", "mf_attention_q8_tc")(
+                _at(q, dt, at, "q"), _at(pages.k, codes, at, "keys"), _at(pages.v, codes, at, "values"),
+                _at(pages.k_scale, f32, at, "key scales"), _at(pages.v_scale, f32, at, "value scales"),
+                offsets + 4 * first, ends + 4 * first, table + 4 * first * table_stride, table_stride, ring,
+                pages.k.shape[0], _at(out, dt, at, "out"), -(-base // 1024) * 1024, tokens, min(some, rows - first),
+                max(1, max_end), stretch, n_heads, n_kv, head_dim, window, scale, fmt, 1 if first == 0 else 0,
+                _at(status, i32, at, "status"), _stream_of(at)), what, 3)
         return
     floats, kernels = attention_q8_plan(tokens, rows, max_row_tokens, span, n_heads, n_kv, head_dim, dt)
     partial = torch.empty(floats, dtype=f32, device=q.device) if floats else None

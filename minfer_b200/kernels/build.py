@@ -47,6 +47,7 @@ LIBRARIES = {
     "outer_scan": ("outer_scan.cu", []),
     "cache_q8": ("cache_q8.cu", []),
     "attention_q8": ("attention_q8.cu", []),
+    "attention_q8_tc": ("attention_q8_tc.cu", []),
     "drafts": ("drafts.cu", []),
 }
 

@@ -307,6 +307,30 @@ def test_offsets_beyond_32_bits(dtype, dim):
     assert torch.equal(out[1][0].cpu(), (small[1][0][1].float() * small[1][1][1].unsqueeze(-1)).to(dtype))
 
 
+@FORMATS
+@pytest.mark.parametrize("heads,kv,dim", [(6, 2, 128), (5, 1, 64)])
+@pytest.mark.parametrize("rows,window,spread", [
+    ([(300, 1000)], 0, 0.0), ([(1, 5), (257, 0), (128, 4000), (129, 127), (2, 0)], 0, 8.0), ([(64, 64)] * 5, 0, 0.0),
+    ([(400, 900), (1, 300), (100, 28)], 130, 8.0), ([(513, 511)], 1, 0.0)], ids=str)
+def test_portions_on_tcgen05(rows, window, spread, heads, kv, dim, fmt, monkeypatch):
+    """As exact as the way that multiplies codes on mma.sync: codes and queries are exact halves there too."""
+    monkeypatch.setattr(K, "q8_reads_back", lambda *a: True)
+    gen, rng = torch.Generator().manual_seed(43), np.random.RandomState(6)
+    new, past = zip(*rows)
+    ends, cu = [n + p for n, p in zip(new, past)], [0] + np.cumsum(new).tolist()
+    ring = -(-(window + max(new) - 1) // PAGE) * PAGE if window else 0
+    table, n_pages = make_table(ends, ring, rng)
+    pages = make_pages(table, n_pages, ends, ring, kv, dim, fmt, gen, spread)
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(torch.bfloat16).to(DEV)
+    for scale in (dim ** -0.5, -0.02, 0.0):
+        got = run_attention(q, pages, cu, ends, table, ring, heads, kv, dim, window, scale)
+        want, *sizes = plain.attention(q, pages, cu, ends, table, ring, heads, kv, window, scale)
+        tol = plain.attention_tolerance(want, *sizes, torch.bfloat16, dim, fmt)
+        assert ((got.double().cpu() - want).abs() <= tol).all()
+        again = run_attention(q, pages, cu, ends, table, ring, heads, kv, dim, window, scale)
+        assert torch.equal(got, again)
+
+
 @pytest.mark.parametrize("window", [0, 90])
 @pytest.mark.parametrize("back", [True, False])
 def test_a_page_table_wider_than_its_rows(window, back, monkeypatch):
