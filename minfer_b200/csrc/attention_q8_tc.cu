@@ -3,28 +3,29 @@
 //
 //   o_i = sum_j p_ij vs_j vc_j / sum_j p_ij,   p_ij = exp(scale q_i . kc_j ks_j - max)
 //
-// Codes are multiplied as they are: an 8-bit code is an exact half, and so is a bfloat16 query brought below
-// 2^15 by a power of two of its vector (elements below 2^-28 of the largest lose bits, then count as
-// zero).  Scales are applied in float32, a key's to its column of scores and a value's to its column of
-// probabilities, and what is rounded to halves for the second product is the probability times its
-// value's scale (off by 2^-11).
+// Keys and values go to the tensor cores as halves, each brought below 2^15 by one power of two of its 128
+// positions (a half has eight times a bfloat16's precision, and scales of neighbouring positions would have to
+// be 2^20 apart to reach the numbers below its normal range); queries are exact halves by a power of two of
+// their vector, and so are probabilities rounded: each of the three is off by 2^-11.  (Codes multiplied as they
+// are, exactly, with the scales applied to scores and probabilities: a row's 128 keys need 384 scales out of
+// shared memory, 3,072 of the 5,200 cycles that a tile then took; this way it takes 3,000.)
 //
 // Three launches:
-//   unpack   the codes that the rows' tokens can see as halves, position behind position (a window over
-//            a ring becomes a stretch), the scales of every 128 keys side by side, the queries as halves
+//   unpack   what the rows' tokens can see, position behind position (a window over a ring becomes a
+//            stretch), and the queries, as halves
 //   attend   a block an SM: items (row, 256 tokens, head), each some tiles of 128 keys, are laid end to
 //            end and dealt out evenly, wherever one item ends and the next begins.  512 tokens of 40 heads
 //            are 80 items, which leave 68 of 148 SMs idle where a block takes whole ones.
 //   join     the items that several blocks have worked on
 //
 // attend is built like the prompts' kernel: a warp issues TMA copies, one the products, and a warpgroup for
-// each of two tiles of 128 queries takes a row of scores a thread out of tensor memory, forms the softmax
-// and puts probabilities back as the A operand of the second product.  Tensor memory: S0 S1 O0 O1.
+// each of two tiles of 128 queries takes a row of scores a thread out of tensor memory, forms the
+// softmax and puts probabilities back as the A operand of the second product.  Tensor memory: S0 S1 O0 O1.
 //
-// The reference of a row's exponentials is the largest weight, m = max_j (s_j + log2 vs_j): the halves are
-// 2^(s_j - m) vs_j <= 2^8, the sum of 2^(s_j - m) is float32 (up to 2^108, since log2 vs counts from -100 on).
+// The reference of a row's exponentials goes by what is rounded: 2^(s_j - m) times the power of two of the tile's
+// values, 2^6 at the largest and up to 2^14 before the reference moves; the sum of 2^(s_j - m) is float32.
 //
-// A scale of NaN marks a vector that was not finite: such a key's score is NaN for the tokens that see it,
+// A scale of NaN marks a vector that was not finite: such a key is NaN, its score too for the tokens that see it,
 // and it is masked for the others; a value's mark is moved to its key, so that zero times NaN is never formed.
 #include "prefill_tc.cuh"
 #include "q8.cuh"
@@ -32,10 +33,11 @@
 #define QT_Q 128              // queries a tile
 #define QT_ITEM 256           // queries an item: two tiles
 #define QT_KEYS 128           // keys a tile
-#define QT_THREADS 384
-#define QT_LAZY 8.0f          // the reference moves when a weight passes it by more than 2^8
+#define QT_THREADS 384        // a warpgroup for copies and products, one for each query tile
+#define QT_BELOW 6.0f         // the reference is put 2^6 below the largest weight, and moves when one passes it by 2^14
+#define QT_ROOM 14.0f
 #define QT_LEAST 4            // least tiles a block takes
-#define QT_SCALES (3 * QT_KEYS)                            // of a tile: ks, log2 vs, vs
+#define QT_LEAST_VALUE (-60)  // values' power of two at least (sums of 2^(s_j - m) stay in float32's range)
 
 struct QtArgs {
     const __nv_bfloat16* q;
@@ -56,7 +58,7 @@ struct QtArgs {
     // scratch
     __half* k16;              // [rows][n_kv][stretch][HD]
     __half* v16;
-    float* scales;            // [rows][n_kv][stretch / 128][ks, log2 vs, vs][128]
+    float2* powers;           // [rows][n_kv][stretch / 128]: the keys' power of two, the values' exponent
     __half* q16;              // [tokens][n_heads][HD]
     float* factor;            // [tokens][n_heads]: scores in powers of two of 2
     int4* first;              // [blocks]: row, item of the row, tile of it, tiles a block
@@ -89,20 +91,20 @@ __device__ __forceinline__ void qt_tiles(const QtArgs& a, const QtRow& r, int q0
 __device__ __forceinline__ int qt_items(const QtRow& r) { return (r.count + QT_ITEM - 1) / QT_ITEM; }
 
 // ------------------------------------------------------------------------------------------
-// unpack: bound by bytes, 1 read and 2 written a code.  A block takes 64 positions of one key/value head, K or V,
+// unpack: bound by bytes, 1 read and 2 written a code.  A block takes 128 positions of one key/value head, K or V,
 // a thread's unit 8 codes (whole lines a warp); the blocks behind them 32 query vectors each, a warp four.
 // ------------------------------------------------------------------------------------------
 #define QU_THREADS 256
 #define QU_VECTORS 32
 template <int FMT, int HD>
-__global__ void __launch_bounds__(QU_THREADS) q8_unpack_kernel(QtArgs a, int n_pages_all) {
+__global__ void __launch_bounds__(QU_THREADS) q8_unpack_kernel(QtArgs a, int n_tiles_all) {
     pdl_launch_dependents();
     const int tid = threadIdx.x;
-    if ((int)blockIdx.x >= n_pages_all) {
+    if ((int)blockIdx.x >= n_tiles_all) {
         // ---- queries ----
         constexpr int PER = HD / 32;                       // elements a lane
         const int warp = tid >> 5, lane = tid & 31;
-        const long long first = (long long)(blockIdx.x - n_pages_all) * QU_VECTORS + warp * 4;
+        const long long first = (long long)(blockIdx.x - n_tiles_all) * QU_VECTORS + warp * 4;
         const long long all = (long long)a.n_tokens * a.n_heads;
         pdl_wait();
         uint32_t w[4][PER / 2];
@@ -149,69 +151,86 @@ __global__ void __launch_bounds__(QU_THREADS) q8_unpack_kernel(QtArgs a, int n_p
         }
         return;
     }
-    // ---- 64 positions of a row ----
-    const int pages = a.stretch / MF_PAGE;
+    // ---- 128 positions of a row ----
+    const int tiles = a.stretch / QT_KEYS;
     int u = blockIdx.x;
     const bool is_v = u & 1;
     u >>= 1;
     const int hk = u % a.n_kv;
     u /= a.n_kv;
-    const int i = u % pages, b = u / pages;
+    const int i = u % tiles, b = u / tiles;
     const QtRow r = qt_row(a, b);
-    const int p0 = r.base + i * MF_PAGE;
-    // (the last tile's second page is read, though it may hold no position, and so is a first tile that holds none)
-    if (r.count == 0 || p0 >= ((max(r.end, r.base + 1) + QT_KEYS - 1) & ~(QT_KEYS - 1))) { pdl_wait(); return; }
+    const int p0 = r.base + i * QT_KEYS;
+    // (a first tile that holds no position is read)
+    if (r.count == 0 || p0 >= max(r.end, r.base + 1)) { pdl_wait(); return; }
     if (tid == 0 && i == 0 && hk == 0 && !is_v && a.seq_end[b] > a.max_end) atomicOr(a.status, MF_STATUS_BAD_POSITION);
-    const int n0 = max(0, r.seen - p0), n1 = min(MF_PAGE, r.end - p0);       // places [n0, n1) are seen
-    const int index = (a.ring > 0 ? p0 % a.ring : p0) >> 6;
-    const int page = index < a.table_stride ? a.page_table[(size_t)b * a.table_stride + index] : -1;
-    const bool there = page >= 0 && page < a.n_pages && n1 > n0;
-    if (!there && n1 > n0 && tid == 0 && hk == 0) atomicOr(a.status, MF_STATUS_BAD_POSITION);
+    const int n0 = max(0, r.seen - p0), n1 = min(QT_KEYS, r.end - p0);       // places [n0, n1) are seen
+    long long from[2];                                                       // the two pages' vectors; -1: none
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int p = p0 + h * MF_PAGE, index = (a.ring > 0 ? p % a.ring : p) >> 6;
+        const bool seen = n1 > h * MF_PAGE && n0 < (h + 1) * MF_PAGE && n1 > n0;
+        const int page = seen && index < a.table_stride ? a.page_table[(size_t)b * a.table_stride + index] : -1;
+        const bool there = page >= 0 && page < a.n_pages;
+        if (seen && !there && tid == 0 && hk == 0) atomicOr(a.status, MF_STATUS_BAD_POSITION);
+        from[h] = there ? ((long long)page * a.n_kv + hk) * MF_PAGE : -1;
+    }
+    __shared__ float scale_s[QT_KEYS];
+    __shared__ unsigned most_s[QT_KEYS / 32];
     pdl_wait();
-    const long long from = there ? ((long long)page * a.n_kv + hk) * MF_PAGE : 0;
-    const uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + from * HD;
-    const long long stretch0 = ((long long)b * a.n_kv + hk) * a.stretch, to = stretch0 + i * MF_PAGE;
-    __half* out = (is_v ? a.v16 : a.k16) + to * HD;
-    constexpr int EACH = MF_PAGE * HD / 8 / QU_THREADS;
+    const uint8_t* codes = is_v ? a.v_codes : a.k_codes;
+    constexpr int EACH = QT_KEYS * HD / 8 / QU_THREADS;
     uint2 w[EACH];
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
-        const int unit = tid + j * QU_THREADS, place = unit / (HD / 8);
-        const bool held = there && place >= n0 && place < n1;                // (what other places hold is anybody's)
-        w[j] = held ? *reinterpret_cast<const uint2*>(codes + unit * 8) : make_uint2(0, 0);
+        // (a page is half of a tile's units)
+        const int unit = tid + (j % (EACH / 2)) * QU_THREADS, place = unit / (HD / 8) + (j / (EACH / 2)) * MF_PAGE;
+        const long long at = from[j / (EACH / 2)];
+        const bool held = at >= 0 && place >= n0 && place < n1;              // (what other places hold is anybody's)
+        w[j] = held ? *reinterpret_cast<const uint2*>(codes + at * HD + unit * 8) : make_uint2(0, 0);
     }
-    if (tid < MF_PAGE) {
-        const bool held = there && tid >= n0 && tid < n1;
-        float ks = held ? a.k_scales[from + tid] : 0.0f, vs = held ? a.v_scales[from + tid] : 0.0f;
-        if (vs != vs) { ks = vs; vs = 1.0f; }
-        float* s = a.scales + stretch0 * 3 + (i >> 1) * QT_SCALES + (i & 1) * MF_PAGE + tid;
-        if (!is_v) {
-            s[0] = ks;
-        } else {
-            s[QT_KEYS] = log2f(fmaxf(vs, 7.9e-31f));                         // (2^-100: values of zeros)
-            s[2 * QT_KEYS] = vs;
-        }
+    if (tid < QT_KEYS) {
+        const long long at = tid < MF_PAGE ? from[0] : from[1];
+        const bool held = at >= 0 && tid >= n0 && tid < n1;
+        const float ks = held ? a.k_scales[at + tid % MF_PAGE] : 0.0f, vs = held ? a.v_scales[at + tid % MF_PAGE] : 0.0f;
+        float x = is_v ? vs : ks;
+        if (is_v && vs != vs) x = 0.0f;
+        if (!is_v && vs != vs) x = vs;
+        scale_s[tid] = x;
+        const unsigned most = __reduce_max_sync(0xffffffffu, x == x ? __float_as_uint(fabsf(x)) : 0u);
+        if ((tid & 31) == 0) most_s[tid >> 5] = most;
     }
+    __syncthreads();
+    // the largest scale to 2^5 .. 2^6, times a code below 2^15
+    const unsigned most = max(max(most_s[0], most_s[1]), max(most_s[2], most_s[3]));
+    const int power = most == 0 ? 0 : min(max((int)(most >> 23) - 127 - 5, is_v ? QT_LEAST_VALUE : -120), 120);
+    const float down = __int_as_float((127 - power) << 23);
+    const long long tile = ((long long)b * a.n_kv + hk) * tiles + i;
+    if (tid == 0) {
+        if (is_v) a.powers[tile].y = (float)power;
+        else a.powers[tile].x = __int_as_float((127 + power) << 23);
+    }
+    __half* out = (is_v ? a.v16 : a.k16) + tile * (QT_KEYS * HD);
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
         const int unit = tid + j * QU_THREADS;
-        const uint32_t x = q8_prepare<FMT>(w[j].x), y = q8_prepare<FMT>(w[j].y);
-        *reinterpret_cast<uint4*>(out + unit * 8) = make_uint4(q8_halves<FMT, false>(x), q8_halves<FMT, true>(x),
-                                                               q8_halves<FMT, false>(y), q8_halves<FMT, true>(y));
+        const float by = scale_s[unit / (HD / 8)] * down;
+        float v[8];
+        q8_floats<FMT>(w[j].x, v);
+        q8_floats<FMT>(w[j].y, v + 4);
+        uint32_t h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const __half2 x = __floats2half2_rn(v[2 * e] * by, v[2 * e + 1] * by);
+            h[e] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+        *reinterpret_cast<uint4*>(out + unit * 8) = make_uint4(h[0], h[1], h[2], h[3]);
     }
 }
 
 // ------------------------------------------------------------------------------------------
 // attend
 // ------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint64_t qt_mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ void qt_lds(uint32_t at, uint64_t& x, uint64_t& y) {        // four floats as two pairs
-    asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(x), "=l"(y) : "r"(at));
-}
 __device__ __forceinline__ uint32_t qt_pack(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -261,20 +280,18 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     uint8_t* q_s = smem;                                // [2 query tiles][NB][128][64]
     uint8_t* k_s = q_s + 2 * T_BYTES;                   // [2 stages]
     uint8_t* v_s = k_s + 2 * T_BYTES;                   // [2 stages]
-    uint8_t* sc_s = v_s + 2 * T_BYTES;                  // [2 stages][QT_SCALES] floats
-    uint64_t* bars = (uint64_t*)(sc_s + 2 * QT_SCALES * 4);
+    uint64_t* bars = (uint64_t*)(v_s + 2 * T_BYTES);
     uint64_t* q_full = bars;
     uint64_t* q_empty = bars + 1;
     uint64_t* k_full = bars + 2;                        // [2 stages] each
     uint64_t* k_empty = bars + 4;
     uint64_t* v_full = bars + 6;
     uint64_t* v_empty = bars + 8;
-    uint64_t* sc_full = bars + 10;
-    uint64_t* sc_empty = bars + 12;                     // 256 arrivals
-    uint64_t* s_full = bars + 14;                       // [2 query tiles] each
-    uint64_t* p_full = bars + 16;                       // 128 arrivals
-    uint64_t* o_done = bars + 18;
-    uint32_t* tmem_slot = (uint32_t*)(bars + 20);
+    uint64_t* s_full = bars + 10;                       // [2 query tiles] each
+    uint64_t* p_half = bars + 12;                       // 128 arrivals: the first 64 keys' weights
+    uint64_t* p_full = bars + 14;                       // 128 arrivals
+    uint64_t* o_done = bars + 16;
+    uint32_t* tmem_slot = (uint32_t*)(bars + 18);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     __shared__ int scan_s[QT_THREADS / 32], at_s[2];
 
@@ -352,9 +369,8 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             fa_bar_init(fa_smem(&k_empty[i]), 1);
             fa_bar_init(fa_smem(&v_full[i]), 1);
             fa_bar_init(fa_smem(&v_empty[i]), 1);
-            fa_bar_init(fa_smem(&sc_full[i]), 1);
-            fa_bar_init(fa_smem(&sc_empty[i]), 256);
             fa_bar_init(fa_smem(&s_full[i]), 1);
+            fa_bar_init(fa_smem(&p_half[i]), 128);
             fa_bar_init(fa_smem(&p_full[i]), 128);
             fa_bar_init(fa_smem(&o_done[i]), 1);
         }
@@ -398,12 +414,6 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 fa_expect_tx(fa_smem(&k_full[st]), T_BYTES);
                 for (int c = 0; c < NB; ++c)
                     fa_tma(fa_smem(k_s + st * T_BYTES + c * BLOCK), &map_k, 64 * c, (tile0 + j) * QT_KEYS, fa_smem(&k_full[st]));
-                if (!fa_wait(fa_smem(&sc_empty[st]), free_parity, abort_flag)) { ok = false; break; }
-                fa_expect_tx(fa_smem(&sc_full[st]), QT_SCALES * 4);
-                asm volatile(
-                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                    ::"r"(fa_smem(sc_s + st * QT_SCALES * 4)), "l"(a.scales + (long long)(tile0 + j) * QT_SCALES),
-                      "r"((uint32_t)(QT_SCALES * 4)), "r"(fa_smem(&sc_full[st])) : "memory");
                 if (!fa_wait(fa_smem(&v_empty[st]), free_parity, abort_flag)) { ok = false; break; }
                 fa_expect_tx(fa_smem(&v_full[st]), T_BYTES);
                 for (int c = 0; c < NB; ++c)
@@ -445,14 +455,19 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 fa_fence_after();
                 const uint32_t v_addr = fa_smem(v_s + (i & 1) * T_BYTES);
                 for (int t = 0; t < tiles; ++t) {
-                    ok = fa_wait(fa_smem(&p_full[t]), (uint32_t)(done[t] & 1), abort_flag);
-                    if (!ok) break;
-                    fa_fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < QT_KEYS / 16; ++ks)
+                    for (int ks = 0; ks < QT_KEYS / 16; ++ks) {
+                        // (the first half of the keys is multiplied while the others' exponentials are formed)
+                        if (ks % (QT_KEYS / 32) == 0) {
+                            ok = fa_wait(fa_smem(ks == 0 ? &p_half[t] : &p_full[t]), (uint32_t)(done[t] & 1), abort_flag);
+                            if (!ok) break;
+                            fa_fence_after();
+                        }
                         fa_mma_ts(tmem + (uint32_t)(TM_O + t * 128), tmem + (uint32_t)(TM_S + t * 128 + ks * 8),
                                   fa_desc_mnmajor(v_addr + (uint32_t)(ks * 16 * 128), BLOCK), idesc_o,
                                   (j > 0 || ks > 0) ? 1u : 0u);
+                    }
+                    if (!ok) break;
                     ++done[t];
                     if (next) issue_qk(t, (i + 1) & 1);
                     else fa_commit(fa_smem(&o_done[t]));
@@ -467,30 +482,35 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-        // ---- softmax: four warps for each query tile, one thread per query row ----
+        // ---- softmax: four warps for each query tile, one thread a query row (two threads, which tell each other
+        // their halves' maxima, take 4,300 cycles a tile where this takes XXX) ----
         const int t = (warp - 4) >> 2;
         const int quarter = warp & 3;                    // the 32 lanes of tensor memory this warp may touch
         const int trow = quarter * 32 + lane;            // row of the tile
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t s_addr = lane_addr + (uint32_t)(TM_S + t * 128);
         const uint32_t o_addr = lane_addr + (uint32_t)(TM_O + t * 128);
-        int i = 0, mine = 0, items = 0;                  // tiles of the block, scores and items of this query tile
+        int mine = 0, items = 0;                         // tiles and items of this query tile
+        // (a warp gives up as one: what follows wants all its lanes)
+        auto wait = [&](uint64_t* bar, int phase) {
+            return (bool)__all_sync(0xffffffffu, fa_wait(fa_smem(bar), (uint32_t)(phase & 1), abort_flag));
+        };
         bool ok = true;
         for (;;) {
             const int q0t = at.group * QT_ITEM + t * QT_Q, qrow = q0t + trow;
             const bool part_of = q0t < at.row.count;     // (the second tile may lie behind the row's tokens)
-            const int start = at.row.end - at.row.count, qpos = start + qrow, wpos = start + q0t + quarter * 32;
+            const int start = at.row.end - at.row.count, wpos = start + q0t + quarter * 32;
             const bool real = qrow < at.row.count;
             const float by = real ? a.factor[(long long)(at.row.tok0 + qrow) * a.n_heads + at.head] : 1.0f;
-            const uint64_t by2 = fa_pack2(by, by);
             float m = -INFINITY, l = 0.0f;
-            for (int j = 0; j < at.part; ++j, ++i) {
-                const uint32_t sc = fa_smem(sc_s + (i & 1) * QT_SCALES * 4);
-                if (!fa_wait(fa_smem(&sc_full[i & 1]), (uint32_t)((i >> 1) & 1), abort_flag)) { ok = false; break; }
-                if (!part_of) { fa_arrive(fa_smem(&sc_empty[i & 1])); continue; }
+            const float2* powers = a.powers + (at.b * a.n_kv + at.head / (a.n_heads / a.n_kv)) * (long long)(a.stretch / QT_KEYS) + at.lo + at.off;
+            float2 power = part_of ? powers[0] : make_float2(1.0f, 0.0f);
+            for (int j = 0; part_of && j < at.part; ++j) {
+                // (factors above 0 keep masked scores at -infinity)
+                const float by_tile = fminf(fmaxf(by * power.x, 1.2e-38f), 3e38f), values = power.y;
+                if (j + 1 < at.part) power = powers[j + 1];
                 // S of this key tile is complete, and with it every earlier product of this query tile
-                if (!fa_wait(fa_smem(&s_full[t]), (uint32_t)(mine & 1), abort_flag)) { ok = false; break; }
-                ++mine;
+                if (!(ok = wait(&s_full[t], mine++))) break;
                 fa_fence_after();
                 const int key0 = at.row.base + (at.lo + at.off + j) * QT_KEYS;
                 const bool need_mask = key0 + QT_KEYS - 1 > wpos || (a.window > 0 && key0 < wpos + 31 - a.window + 1);
@@ -498,99 +518,76 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
                 for (int c0 = 0; c0 < QT_KEYS; c0 += 32) fa_ld32(s_addr + (uint32_t)c0, sr + c0);
                 fa_wait_ld();
-                // scores in the codes' units times the keys' scales
-#pragma unroll
-                for (int e = 0; e < QT_KEYS; e += 4) {
-                    uint64_t k01, k23;
-                    float x0, x1, x2, x3;
-                    qt_lds(sc + e * 4, k01, k23);
-                    fa_unpack2(qt_mul2(qt_pair(sr + e), k01), x0, x1);
-                    fa_unpack2(qt_mul2(qt_pair(sr + e + 2), k23), x2, x3);
-                    sr[e] = __float_as_uint(x0); sr[e + 1] = __float_as_uint(x1);
-                    sr[e + 2] = __float_as_uint(x2); sr[e + 3] = __float_as_uint(x3);
-                }
                 if (need_mask) {
+                    const int qpos = start + qrow;
                     const int first = a.window > 0 ? qpos - a.window + 1 - key0 : 0, last = qpos - key0;
 #pragma unroll
                     for (int e = 0; e < QT_KEYS; ++e)
                         if (e > last || e < first) sr[e] = 0xff800000u;              // -infinity
                 }
-                // the largest weight, with four chains of three-input maxima
+                // the largest score, with four chains of three-input maxima
                 float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < QT_KEYS; e += 8) {
-                    uint64_t v01, v23, v45, v67;
-                    float y0, y1, y2, y3, y4, y5, y6, y7;
-                    qt_lds(sc + QT_KEYS * 4 + e * 4, v01, v23);
-                    qt_lds(sc + QT_KEYS * 4 + e * 4 + 16, v45, v67);
-                    fa_unpack2(fa_fma2(qt_pair(sr + e), by2, v01), y0, y1);
-                    fa_unpack2(fa_fma2(qt_pair(sr + e + 2), by2, v23), y2, y3);
-                    fa_unpack2(fa_fma2(qt_pair(sr + e + 4), by2, v45), y4, y5);
-                    fa_unpack2(fa_fma2(qt_pair(sr + e + 6), by2, v67), y6, y7);
-                    mx0 = fa_max3(mx0, y0, y1);
-                    mx1 = fa_max3(mx1, y2, y3);
-                    mx2 = fa_max3(mx2, y4, y5);
-                    mx3 = fa_max3(mx3, y6, y7);
+                    mx0 = fa_max3(mx0, __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+                    mx1 = fa_max3(mx1, __uint_as_float(sr[e + 2]), __uint_as_float(sr[e + 3]));
+                    mx2 = fa_max3(mx2, __uint_as_float(sr[e + 4]), __uint_as_float(sr[e + 5]));
+                    mx3 = fa_max3(mx3, __uint_as_float(sr[e + 6]), __uint_as_float(sr[e + 7]));
                 }
-                const float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
-                const bool jump = m == -INFINITY ? m_tile > -INFINITY : m_tile - m > QT_LAZY;
-                const float m_new = jump ? m_tile : m;
+                const float m_tile = fmaf(fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)), by_tile, values);
+                const bool jump = m == -INFINITY ? m_tile > -INFINITY : m_tile - m > QT_ROOM;
+                const float m_new = jump ? m_tile - QT_BELOW : m;
                 const float m_off = m_new == -INFINITY ? 0.0f : m_new;
-                const float corr = m == -INFINITY ? 0.0f : exp2f(m - m_off);
                 // the output so far is rescaled only if the reference moved for some row of this warp
                 if (j > 0 && __any_sync(0xffffffffu, jump)) {
+                    const float corr = jump ? (m == -INFINITY ? 0.0f : exp2f(m - m_off)) : 1.0f;
+                    l *= corr;
 #pragma unroll 1
                     for (int c0 = 0; c0 < HD; c0 += 32) {
                         uint32_t r[32];
                         fa_ld32(o_addr + (uint32_t)c0, r);
                         fa_wait_ld();
-                        if (jump) {
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
-                        }
+                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
                         fa_st32(o_addr + (uint32_t)c0, r);
                     }
                 }
-                if (jump) l *= corr;
                 m = m_new;
-                // exponentials, their sum, and times the values' scales as halves in the first 64 columns of S
+                // weights 2^(s - m) times the values' power of two, their sum, and as halves into the first 64 columns
+                // of S
                 uint64_t l01 = 0, l23 = 0;               // four zeros
-                const uint64_t off2 = fa_pack2(-m_off, -m_off);
-                uint32_t pk[QT_KEYS / 2];
+                const uint64_t by2 = fa_pack2(by_tile, by_tile), off2 = fa_pack2(values - m_off, values - m_off);
 #pragma unroll
-                for (int e = 0; e < QT_KEYS; e += 4) {
-                    uint64_t v01, v23;
-                    float x0, x1, x2, x3;
-                    qt_lds(sc + 2 * QT_KEYS * 4 + e * 4, v01, v23);
-                    fa_unpack2(fa_fma2(qt_pair(sr + e), by2, off2), x0, x1);
-                    fa_unpack2(fa_fma2(qt_pair(sr + e + 2), by2, off2), x2, x3);
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x0));
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x1));
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x2));
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x3));
-                    const uint64_t p01 = fa_pack2(x0, x1), p23 = fa_pack2(x2, x3);
-                    l01 = fa_add2(l01, p01);
-                    l23 = fa_add2(l23, p23);
-                    fa_unpack2(qt_mul2(p01, v01), x0, x1);
-                    fa_unpack2(qt_mul2(p23, v23), x2, x3);
-                    pk[e >> 1] = qt_pack(x0, x1);
-                    pk[(e >> 1) + 1] = qt_pack(x2, x3);
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t pk[QT_KEYS / 4];
+#pragma unroll
+                    for (int g = 0; g < QT_KEYS / 2; g += 4) {
+                        const int e = h * (QT_KEYS / 2) + g;
+                        float x0, x1, x2, x3;
+                        fa_unpack2(fa_fma2(qt_pair(sr + e), by2, off2), x0, x1);
+                        fa_unpack2(fa_fma2(qt_pair(sr + e + 2), by2, off2), x2, x3);
+                        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x0));
+                        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x1));
+                        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x2));
+                        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x3));
+                        l01 = fa_add2(l01, fa_pack2(x0, x1));
+                        l23 = fa_add2(l23, fa_pack2(x2, x3));
+                        pk[g >> 1] = qt_pack(x0, x1);
+                        pk[(g >> 1) + 1] = qt_pack(x2, x3);
+                    }
+                    fa_st32(s_addr + (uint32_t)(h * (QT_KEYS / 4)), pk);
+                    fa_wait_st();
+                    fa_fence_before();
+                    fa_arrive(fa_smem(h == 0 ? &p_half[t] : &p_full[t]));
                 }
-                fa_arrive(fa_smem(&sc_empty[i & 1]));
                 float l0, l1, l2, l3;
                 fa_unpack2(l01, l0, l1);
                 fa_unpack2(l23, l2, l3);
-                l += (l0 + l1) + (l2 + l3);
-#pragma unroll
-                for (int c0 = 0; c0 < QT_KEYS / 2; c0 += 32) fa_st32(s_addr + (uint32_t)c0, pk + c0);
-                fa_wait_st();
-                fa_fence_before();
-                fa_arrive(fa_smem(&p_full[t]));
+                l = fmaf((l0 + l1) + (l2 + l3), exp2f(-values), l);
             }
             // ---- the item's result, or a part of it ----
             if (ok && part_of) {
-                if (!fa_wait(fa_smem(&o_done[t]), (uint32_t)(items & 1), abort_flag)) break;
-                ++items;
+                if (!wait(&o_done[t], items++)) break;
                 fa_fence_after();
                 const bool whole = at.off == 0 && at.part == at.n;
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -728,7 +725,7 @@ static long long qt_layout(QtArgs* a, uint8_t* base, int n_tokens, int n_rows, i
     a->slots = (float*)take(2LL * blocks * (long long)qt_slot_floats(hd) * 4);
     a->k16 = (__half*)take(vectors * hd * 2);
     a->v16 = (__half*)take(vectors * hd * 2);
-    a->scales = (float*)take(vectors * 12);
+    a->powers = (float2*)take(vectors / QT_KEYS * 8);
     return at;
 }
 // Bytes of scratch of a call over `n_rows` rows whose tokens see `stretch` positions (a multiple of 128).
@@ -743,7 +740,7 @@ template <int HD> static int qt_launch(const QtArgs& a, int fmt, cudaStream_t st
     if (int e = qt_map(&mq, a.q16, a.n_tokens, (long long)a.n_heads * HD)) return e;
     if (int e = qt_map(&mk, a.k16, vectors, HD)) return e;
     if (int e = qt_map(&mv, a.v16, vectors, HD)) return e;
-    constexpr int used = (HD / 64) * 16384 * 6 + 1024 + 2 * QT_SCALES * 4 + 256;
+    constexpr int used = (HD / 64) * 16384 * 6 + 1024 + 256;
     // (tensor memory is allocated whole: no other block with some may share the SM)
     constexpr int smem = used > MF_TMEM_SMEM_ALONE ? used : MF_TMEM_SMEM_ALONE;
     static bool opened[64] = {};
@@ -754,12 +751,12 @@ template <int HD> static int qt_launch(const QtArgs& a, int fmt, cudaStream_t st
             return (int)e;
         if (dev >= 0 && dev < 64) opened[dev] = true;
     }
-    const long long pages = vectors / MF_PAGE * 2;
+    const long long tiles = vectors / QT_KEYS * 2;
     const long long queries = a.with_q ? ((long long)a.n_tokens * a.n_heads + QU_VECTORS - 1) / QU_VECTORS : 0;
-    if (pages + queries > 0x7fffffffLL) return MF_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)(pages + queries));
-    if (fmt == MF_Q8_E4M3) mf_launch(q8_unpack_kernel<MF_Q8_E4M3, HD>, grid, dim3(QU_THREADS), 0, stream, a, (int)pages);
-    else mf_launch(q8_unpack_kernel<MF_Q8_INT8, HD>, grid, dim3(QU_THREADS), 0, stream, a, (int)pages);
+    if (tiles + queries > 0x7fffffffLL) return MF_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)(tiles + queries));
+    if (fmt == MF_Q8_E4M3) mf_launch(q8_unpack_kernel<MF_Q8_E4M3, HD>, grid, dim3(QU_THREADS), 0, stream, a, (int)tiles);
+    else mf_launch(q8_unpack_kernel<MF_Q8_INT8, HD>, grid, dim3(QU_THREADS), 0, stream, a, (int)tiles);
     if (int e = MF_LAUNCH_CHECK()) return e;
     const int blocks = mf_sm_count();
     mf_launch(attention_q8_tc_kernel<HD>, dim3(blocks), dim3(QT_THREADS), smem, stream, mq, mk, mv, a);
