@@ -390,9 +390,10 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     fa_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // Registers: compiled for 168 a thread; the first warpgroup gives most of its share to the other two.
+    // Registers: compiled for 168 a thread, 64,512 in all; the first warpgroup gives half of its share to the other
+    // two: 128 * 88 + 256 * 208 = 64,512.  (At 56 its two walks through the items spill: 3 % slower.)
     if (warp < 4) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
       if (warp == 0 && elect_one()) {
         // ---- TMA producer: `i` counts the block's tiles, `s` its items ----
         int i = 0;
@@ -481,7 +482,7 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
       }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ---- softmax: four warps for each query tile, one thread a query row (two threads, which tell each other
         // their halves' maxima, take 4,300 cycles a tile where this takes XXX) ----
         const int t = (warp - 4) >> 2;

@@ -1286,25 +1286,37 @@ def attention_q8_plan(n_tokens: int, n_rows: int, max_row_tokens: int, span: int
     return got
 
 
-Q8_PORTION_BYTES = 2 << 30      # of pages read back at a time
+Q8_PORTION_BYTES = 2 << 30      # of keys and values unpacked at a time
 
 
-def q8_reads_back(tokens: int, rows: int, max_row_tokens: int, span: int, n_heads: int, n_kv: int, head_dim: int,
+def q8_on_tcgen05(tokens: int, rows: int, max_row_tokens: int, span: int, n_heads: int, n_kv: int, head_dim: int,
                   sms: int) -> bool:
-    """Whether attention over 8-bit pages reads them back into bfloat16 and runs the tcgen05 kernel of portions
-    (query tiles of 256 tokens of one head) instead of multiplying codes on mma.sync (all heads of a group
-    and all tokens of a row share the keys).  Both times are estimated from what they were measured at, for
-    rows of ``span`` positions: the tcgen05 kernel walks a row's keys at 14 ns each (12 at head size 64) in as
-    many rounds as its blocks need of the SMs, behind 3 bytes a code at 5 TB/s; the other does 225 TFLOP/s
-    (165).  Measured on both sides, us, codes against read back, 28 heads / 4 of 128 over 4,000 positions: 1 row
-    of 128 tokens 54 / 70, of 256 92 / 77; 8 rows of 32 90 / 142, of 128 290 / 152; 14 / 2 of 64: 1 row of 256
-    41 / 70, 8 rows of 64 68 / 59, 32 rows of 32 109 / 215, of 64 187 / 217, of 128 345 / 226."""
+    """Whether attention over 8-bit pages takes the tcgen05 kernel of portions (csrc/attention_q8_tc.cu: 256 tokens
+    of one head an item, three launches, keys and values unpacked first) instead of multiplying codes on mma.sync
+    (csrc/attention_q8.cu: all heads of a group share the keys, 32 rows of them a block).  Both times are
+    estimated from what they were measured at, for rows of ``span`` positions.  tcgen05: 18 us, 1.65 us a tile of
+    128 keys and block (1.35 at head size 64; 2.3 and 1.85 where an item has a second tile of queries), two and a half
+    tiles more an item, 3 bytes a code at 5 TB/s.  mma.sync: 225 TFLOP/s (165) of the blocks that the call fills, 10 us
+    for every further round of them.  Measured, us, mma.sync / tcgen05: 28 heads, 4 of 128: 1 row of 64 tokens behind
+    4,000 33 / 33, of 256 92 / 43, of 1,024 339 / 89; 8 rows of 32 90 / 131, of 64 159 / 130, of 256 570 / 165; 32 rows of
+    64 behind none 94 / 62; 14 / 2 of 64, behind 4,000: 1 row of 128 25 / 25, of 256 41 / 31, 8 rows of 32 39 / 59, of 64
+    69 / 59, of 256 195 / 74."""
     if max_row_tokens < 32:
         return False
-    wide = head_dim == 128
-    rounds = -(-n_heads * rows * -(-max_row_tokens // 256) // sms)
-    back = rounds * span * (14e-9 if wide else 12e-9) + rows * span * n_kv * head_dim * 6 / 5e12 + 8e-6
-    codes = 4.0 * tokens * span * n_heads * head_dim / (225e12 if wide else 165e12) + 4e-6
+    wide, group = head_dim == 128, n_heads // n_kv
+    # (tensor cores' rates and times a tile: head size 128, then 64)
+    tile = (2.3e-6 if max_row_tokens > 128 else 1.65e-6) if wide else (1.85e-6 if max_row_tokens > 128 else 1.35e-6)
+    units = n_heads * rows * -(-max_row_tokens // 256) * (span / 128 + 2.5)
+    back = 18e-6 + max(1.0, units / sms) * tile + 6 * rows * span * n_kv * head_dim / 5e12
+    blocks, held = rows * n_kv * -(-max_row_tokens * group // 32), sms * (2 if wide else 3)
+    split = 1
+    while split < 8 and 2 * split * blocks <= held:
+        split *= 2
+    full = 1.0 if 2 * split * blocks <= held else min(1.0, split * blocks / held)
+    if not wide:                      # (three blocks an SM: two of them run faster)
+        full = max(full, 0.7)
+    codes = (4e-6 + 4.0 * tokens * span * n_heads * head_dim / ((225e12 if wide else 165e12) * full) +
+             10e-6 * max(0.0, blocks / held - 1.0))
     return back < codes
 
 
@@ -1318,8 +1330,9 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
     to its own (the last ``window`` of them where that is not 0) and reads zeros if there is none.
     ``max_row_tokens``: the most tokens a row brings; ``max_end``: a bound of ``seq_end`` (it sizes the splits).
     A page that a token would see and its row has not sets status bit 2; what such a row reads is undefined, but
-    nothing outside the pages is touched and other rows are not.  Long portions are read back into bfloat16 first
-    (``q8_reads_back``), in scratch of at most ``Q8_PORTION_BYTES`` or one row's pages."""
+    nothing outside the pages is touched and other rows are not.  Portions of many tokens run
+    on tcgen05 (``q8_on_tcgen05``), keys and values rounded to halves, over scratch of at most ``Q8_PORTION_BYTES``
+    and what one row, the queries and the blocks' results take."""
     what = "attention_paged_q8"
     rows, tokens = seq_end.numel(), q.shape[0]
     if n_kv < 1 or n_heads < 1 or n_heads % n_kv != 0:
@@ -1341,7 +1354,7 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
     span = max_end
     if window > 0:                    # from a page's border on
         span = min(span, window + max_row_tokens + PAGE - 1)
-    if max_row_tokens >= 32 and dt is torch.bfloat16 and head_dim in (64, 128) and q8_reads_back(
+    if max_row_tokens >= 32 and dt is torch.bfloat16 and head_dim in (64, 128) and q8_on_tcgen05(
             tokens, rows, max_row_tokens, span, n_heads, n_kv, head_dim, sm_count(q.device)):
         # positions of a row in the scratch: what its tokens can see, in tiles of 128 from a tile's border on
         reach = max(1, max_end)

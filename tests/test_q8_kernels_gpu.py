@@ -314,7 +314,7 @@ def test_offsets_beyond_32_bits(dtype, dim):
     ([(400, 900), (1, 300), (100, 28)], 130, 8.0), ([(513, 511)], 1, 0.0)], ids=str)
 def test_portions_on_tcgen05(rows, window, spread, heads, kv, dim, fmt, monkeypatch):
     """Keys, values and probabilities are halves there: eight times as exact as bfloat16."""
-    monkeypatch.setattr(K, "q8_reads_back", lambda *a: True)
+    monkeypatch.setattr(K, "q8_on_tcgen05", lambda *a: True)
     gen, rng = torch.Generator().manual_seed(43), np.random.RandomState(6)
     new, past = zip(*rows)
     ends, cu = [n + p for n, p in zip(new, past)], [0] + np.cumsum(new).tolist()
@@ -337,7 +337,7 @@ def test_portions_on_tcgen05(rows, window, spread, heads, kv, dim, fmt, monkeypa
 def test_a_page_table_wider_than_its_rows(window, back, monkeypatch):
     """Places that no position of a row can lie in cost nothing and change nothing; a length beyond ``max_end``
     is reported where that sizes what is read back."""
-    monkeypatch.setattr(K, "q8_reads_back", lambda *a: back)
+    monkeypatch.setattr(K, "q8_on_tcgen05", lambda *a: back)
     heads, kv, dim, fmt = 6, 2, 128, torch.int8
     gen, rng = torch.Generator().manual_seed(41), np.random.RandomState(6)
     ends, cu = [140, 75, 33], [0, 40, 108, 141]
@@ -396,7 +396,7 @@ def test_portions_that_are_read_back(rows, window, heads, kv, dim, fmt, at_a_tim
     """The other way to attend, which long portions take: the same result, NaN with those who see it only
     (a value of NaN in a later token, in another row, in a place no row sees), in one go and some rows at a
     time."""
-    monkeypatch.setattr(K, "q8_reads_back", lambda *a: True)
+    monkeypatch.setattr(K, "q8_on_tcgen05", lambda *a: True)
     gen, rng = torch.Generator().manual_seed(41), np.random.RandomState(6)
     new, past = zip(*rows)
     ends = [n + p for n, p in zip(new, past)]
