@@ -9,7 +9,8 @@
 // the codes are multiplied as they are.  A token that sees nothing gets zeros.
 //
 // All tokens of a row and all query heads of a key/value head share the keys: their rows are the rows of
-// one matrix product, r = token * group + head.
+// one matrix product, r = token * group + head.  (Portions of many tokens have a kernel on tcgen05,
+// attention_q8_tc.cu.)
 #include "q8.cuh"
 
 #include <cooperative_groups.h>
@@ -31,6 +32,7 @@ struct AttnQ8Args {
     int max_end;                   // positions that the page table has room for
     int n_splits;                  // parts that a row's pages are shared out to
     int q_groups;                  // blocks along the longest row's matrix rows
+    int block_rows;                // matrix rows a block takes
     float scale;
     unsigned* status;
 };
@@ -93,6 +95,13 @@ __device__ __forceinline__ float lds32(uint32_t at) {
 // of 2^(s_j - m) is float32.  m is moved up (and outputs rescaled) only when a weight passes it by more than
 // 2^10: nothing is near overflow until then, and the usual step needs one vote and no exchange between
 // lanes.
+//
+// Bound by bytes where rows are few and caches long: 64 sequences of 4,097 to 8,192 positions, one token each, 28
+// heads, 4 of keys, 128: 65 us, 5.3 TB/s (0.81 of a copy), two thirds of that the 61 us of one launch whose
+// blocks wait for their first pages 3 us.  Where rows are many, a step of 16 keys takes a warp about 1,650 clocks
+// at 24 rows (16 sequences with 4 drafts each over 2,000 positions: 30.8 us): its loads, conversions, products and
+// exponentials follow one another, and two or three warps a scheduler do not hide them all.  Short calls are
+// latency (8 sequences of 500 to 2,048 positions: 10.3 us).
 //
 // Layouts: row r of a score tile is key 4 (r' >> 1) + 2 (r >> 3) + (r & 1), r' = r & 7, of the step's 16, so that
 // the keys a thread multiplies values of are the four from 4 t on.  Both operands of a score see the same
@@ -785,17 +794,70 @@ __global__ void __launch_bounds__(AQ_JOIN_WARPS * 32) attention_q8_join_kernel(A
 // FP32 pipe (the true 32-bit path).  A block takes up to eight matrix rows of one key/value head; 32
 // keys at a time are turned into float32 codes in shared memory once for all of them, lanes are keys
 // in the scores and dimensions in the sums; a warp's two rows share what it reads of keys and values.  Bound by
-// the shared-memory reads of the products.  ND: 32 dimensions a lane has one of, rounded up to 1, 2, 4 or 8.
+// the shared-memory reads of the products: 16 sequences over 4,000 positions, 28 heads, 4 of keys, 128: 146 us, 6
+// TFLOP/s; few rows by latency (4 of 1 to 3 tokens over 60 to 611: 14.4 us, the join 3 of them).  ND: 32 dimensions a lane has one of, rounded up to 1, 2, 4 or 8.
 // ------------------------------------------------------------------------------------------
 #define AG_WARPS 4
 #define AG_ROWS 8
 #define AG_KEYS 32
 
+// KEYS positions' codes, from vector `at` of the pages on, as float values or halves (exact both): keys in rows of
+// hs elements, values of hd.  A thread's unit is 4 codes, so that stores meet every bank; places outside [n0, n1) are zeros (what they hold
+// is anybody's).  `by_row`: 2^32 / (hd / 4), rounded up: a unit's row by one multiplication.
+template <int FMT, int KEYS, typename E>
+__device__ __forceinline__ void ag_load(const AttnQ8Args& a, long long at, int n0, int n1, E* k_s, int hs, E* v_s,
+                                        unsigned by_row) {
+    const int hd = a.hd, upr = hd >> 2, units = KEYS * upr;
+#pragma unroll 1
+    for (int u0 = threadIdx.x; u0 < 2 * units; u0 += 8 * 128) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int u = u0 + j * 128, v = u >= units ? u - units : u, r = (int)__umulhi((unsigned)v, by_row);
+            w[j] = 0;
+            if (u < 2 * units && r >= n0 && r < n1)
+                w[j] = reinterpret_cast<const uint32_t*>((u >= units ? a.v_codes : a.k_codes) + at * hd)[v];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int u = u0 + j * 128, v = u >= units ? u - units : u, r = (int)__umulhi((unsigned)v, by_row);
+            if (u >= 2 * units) continue;
+            E* to = u >= units ? v_s + 4 * v : k_s + r * hs + 4 * (v - r * upr);
+            if constexpr (sizeof(E) == 4) {
+                float f[4];
+                q8_floats<FMT>(w[j], f);
+                *reinterpret_cast<float4*>(to) = make_float4(f[0], f[1], f[2], f[3]);
+            } else {
+                const uint32_t x = q8_prepare<FMT>(w[j]);
+                *reinterpret_cast<uint2*>(to) = make_uint2(q8_halves<FMT, false>(x), q8_halves<FMT, true>(x));
+            }
+        }
+    }
+}
+// ROWS matrix rows' queries times the scale, zeros behind the last; place_s: where a row lies among q and out.
+template <typename T, int ROWS>
+__device__ __forceinline__ void ag_queries(const AttnQ8Args& a, int tok0, int hk, int r0, int rows, size_t* place_s, float* q_s) {
+    const int G = a.n_heads / a.n_kv, hd = a.hd;
+    if (threadIdx.x < ROWS) {
+        const int r = r0 + threadIdx.x, token = r / G;
+        place_s[threadIdx.x] = (size_t)(tok0 + token) * a.n_heads + hk * G + r - token * G;
+    }
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < ROWS / 4; ++j) {
+        const int r = warp + 4 * j;
+        const T* from = (const T*)a.q + place_s[r] * hd;
+        for (int d = lane; d < hd; d += 32) q_s[r * hd + d] = r < rows ? to_f32(from[d]) * a.scale : 0.0f;
+    }
+}
+
 template <typename T, int FMT, int ND>
-__global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(AttnQ8Args a) {
+__global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(AttnQ8Args a, unsigned by_row) {
     extern __shared__ __align__(16) uint8_t ag_smem[];
     pdl_launch_dependents();
-    const int hd = a.hd, hs = hd + 1;                      // odd rows: a column of keys meets every bank
+    __shared__ size_t place_s[AG_ROWS];
+    const int hd = a.hd, hs = hd + 4;                      // rows of an odd number of 16 bytes: lanes meet every bank
     float* k_s = (float*)ag_smem;                          // [AG_KEYS][hs]
     float* v_s = k_s + AG_KEYS * hs;                       // [AG_KEYS][hd]
     float* q_s = v_s + AG_KEYS * hd;                       // [AG_ROWS][hd]
@@ -817,14 +879,9 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
     const int lo = max(lo_all, base), hi = min(last + 1, base + chunk);
     const int* table = a.page_table + (size_t)b * a.table_stride;
     pdl_wait();
-    for (int i = tid; i < rows * hd; i += AG_WARPS * 32) {
-        const int r = i / hd, d = i - r * hd, token = (r0 + r) / G, head = hk * G + (r0 + r) - token * G;
-        q_s[i] = to_f32(((const T*)a.q)[((size_t)(tok0 + token) * a.n_heads + head) * hd + d]) * a.scale;
-    }
+    ag_queries<T, AG_ROWS>(a, tok0, hk, r0, rows, place_s, q_s);
     constexpr int RW = AG_ROWS / AG_WARPS;                 // rows a warp
     static_assert(RW == 2, "a warp's weights are read as pairs");
-    // rows that are not there multiply zeros
-    for (int i = tid + rows * hd; i < AG_ROWS * hd; i += AG_WARPS * 32) q_s[i] = 0.0f;
     float m_r[RW], l_r[RW], acc[RW][ND];
     int lo_w[RW], hi_w[RW];
 #pragma unroll
@@ -846,21 +903,7 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
         }
         const long long at = ((long long)page * a.n_kv + hk) * MF_PAGE + (j0 & (MF_PAGE - 1));
         __syncthreads();                                   // the step before is done with the buffers
-        for (int i = tid; i < 2 * AG_KEYS * hd / 16; i += AG_WARPS * 32) {
-            const bool is_v = i >= AG_KEYS * hd / 16;
-            const int u = is_v ? i - AG_KEYS * hd / 16 : i, r = u * 16 / hd, d = u * 16 - r * hd;
-            uint4 w = *reinterpret_cast<const uint4*>((is_v ? a.v_codes : a.k_codes) + at * hd + u * 16);
-            if (j0 + r < lo || j0 + r >= hi) w = make_uint4(0, 0, 0, 0);       // anybody's
-            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-            float* to = is_v ? v_s + r * hd + d : k_s + r * hs + d;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float f[4];
-                q8_floats<FMT>(x[j], f);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) to[4 * j + e] = f[e];
-            }
-        }
+        ag_load<FMT, AG_KEYS>(a, at, lo - j0, hi - j0, k_s, hs, v_s, by_row);
         if (tid < AG_KEYS) ks_s[tid] = a.k_scales[at + tid];
         else if (tid < 2 * AG_KEYS) vs_s[tid - AG_KEYS] = a.v_scales[at + tid - AG_KEYS];
         __syncthreads();
@@ -879,12 +922,12 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
         for (int i = 0; i < RW; ++i) dot[i][0] = dot[i][1] = dot[i][2] = dot[i][3] = 0.0f;
 #pragma unroll 4
         for (int d = 0; d < hd; d += 4) {
-            const float k0 = kr[d], k1 = kr[d + 1], k2 = kr[d + 2], k3 = kr[d + 3];
+            const float4 k4 = *reinterpret_cast<const float4*>(kr + d);
 #pragma unroll
             for (int i = 0; i < RW; ++i) {
                 const float4 q4 = *reinterpret_cast<const float4*>(qr + i * hd + d);
-                dot[i][0] = fmaf(q4.x, k0, dot[i][0]); dot[i][1] = fmaf(q4.y, k1, dot[i][1]);
-                dot[i][2] = fmaf(q4.z, k2, dot[i][2]); dot[i][3] = fmaf(q4.w, k3, dot[i][3]);
+                dot[i][0] = fmaf(q4.x, k4.x, dot[i][0]); dot[i][1] = fmaf(q4.y, k4.y, dot[i][1]);
+                dot[i][2] = fmaf(q4.z, k4.z, dot[i][2]); dot[i][3] = fmaf(q4.w, k4.w, dot[i][3]);
             }
         }
 #pragma unroll
@@ -917,8 +960,7 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
     for (int i = 0; i < RW; ++i) {
         const int r = warp * RW + i;
         if (r >= rows) continue;
-        const int token = (r0 + r) / G, head = hk * G + (r0 + r) - token * G;
-        const size_t th = (size_t)(tok0 + token) * a.n_heads + head;
+        const size_t th = place_s[r];
         if (a.n_splits > 1) {
             float* p = a.partial + (th * a.n_splits + split) * (hd + 2);
             if (lane == 0) {
@@ -934,6 +976,175 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
 #pragma unroll
             for (int d = 0; d < ND; ++d)
                 if (lane + 32 * d < hd) ((T*)a.out)[th * hd + lane + 32 * d] = from_f32<T>(acc[i][d] * inv);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// The same for many matrix rows: a block takes 32 rows and 64 keys at a time.  Scores and outputs are formed in
+// tiles of registers, since shared memory gives a warp 128 bytes a clock however few addresses it asks for: a thread
+// has 4 rows by 4 keys and 4 rows by hd / 16 dimensions; sixteen lanes of a warp share four rows, so weights pass
+// between them without a barrier of the block.  Codes lie in shared memory as halves (exact), which lets three
+// blocks share an SM (as floats two: 16 sequences of 4 tokens behind 2,000, 40 heads, 8 of keys, 128: 246 us, 378
+// with floats).  12 TFLOP/s of 72: loads are waited for in front of each page, and three blocks do not hide that.
+// NJ: 64 dimensions, rounded up.
+// ------------------------------------------------------------------------------------------
+#define AM_ROWS 32
+#define AM_KEYS 64
+#define AM_LEAST 12            // rows beyond which a block takes 32
+__device__ __forceinline__ float4 am_floats(const __half* p) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(x.x, x.y, y.x, y.y);
+}
+template <typename T, int FMT, int NJ>
+__global__ void __launch_bounds__(128) attention_q8_rows_kernel(AttnQ8Args a, unsigned by_row) {
+    extern __shared__ __align__(16) uint8_t ag_smem[];
+    pdl_launch_dependents();
+    const int hd = a.hd, hs = hd + 4;                      // rows of an odd number of 8 bytes: lanes meet every bank
+    __half* k_s = (__half*)ag_smem;                        // [AM_KEYS][hs]
+    __half* v_s = k_s + AM_KEYS * hs;                      // [AM_KEYS][hd]
+    float* q_s = (float*)(v_s + AM_KEYS * hd);             // [AM_ROWS][hd]
+    float* ks_s = q_s + AM_ROWS * hd;                      // [AM_KEYS] each
+    float* vs_s = ks_s + AM_KEYS;
+    float4* p_s = (float4*)(vs_s + AM_KEYS);               // [8][AM_KEYS]: the weights of four rows
+    __shared__ size_t place_s[AM_ROWS];
+    const int tid = threadIdx.x, rg = tid >> 4, kg = tid & 15;
+    const int split = blockIdx.x, hk = blockIdx.y / a.q_groups, qg = blockIdx.y - hk * a.q_groups, b = blockIdx.z;
+    const int G = a.n_heads / a.n_kv;
+    int tok0, count, end;
+    aq_bounds(a, b, &tok0, &count, &end);
+    const int r0 = qg * AM_ROWS, rows = min(AM_ROWS, count * G - r0);
+    if (rows <= 0) { pdl_wait(); return; }
+    const int first = end - count + r0 / G, last = end - count + (r0 + rows - 1) / G;
+    const int lo_all = a.window > 0 ? max(0, first - a.window + 1) : 0;
+    const int base0 = lo_all & ~(MF_PAGE - 1), pages = max(0, (last - base0 + MF_PAGE) / MF_PAGE);
+    const int chunk = (pages + a.n_splits - 1) / a.n_splits * MF_PAGE;
+    const int base = base0 + split * chunk;
+    const int lo = max(lo_all, base), hi = min(last + 1, base + chunk);
+    const int* table = a.page_table + (size_t)b * a.table_stride;
+    pdl_wait();
+    ag_queries<T, AM_ROWS>(a, tok0, hk, r0, rows, place_s, q_s);
+    float m_r[4], l_r[4], acc[4][4 * NJ];
+    int lo_w[4], hi_w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        m_r[i] = AQ_NEG; l_r[i] = 0.0f;
+        const int r = rg * 4 + i;
+        hi_w[i] = r < rows ? end - count + (r0 + r) / G + 1 : 0;
+        lo_w[i] = r < rows && a.window > 0 ? max(0, hi_w[i] - a.window) : 0;
+#pragma unroll
+        for (int d = 0; d < 4 * NJ; ++d) acc[i][d] = 0.0f;
+    }
+    for (int j0 = lo & ~(AM_KEYS - 1); j0 < hi; j0 += AM_KEYS) {             // a page a step
+        const int index = (a.ring > 0 ? j0 % a.ring : j0) >> 6;
+        const int page = index < a.table_stride ? table[index] : -1;
+        if (page < 0 || page >= a.n_pages) {                                 // (uniform over the block)
+            if (tid == 0) atomicOr(a.status, MF_STATUS_BAD_POSITION);
+            continue;
+        }
+        const long long at = ((long long)page * a.n_kv + hk) * MF_PAGE;
+        __syncthreads();                                   // the step before is done with the buffers
+        ag_load<FMT, AM_KEYS>(a, at, lo - j0, hi - j0, k_s, hs, v_s, by_row);
+        if (tid < AM_KEYS) ks_s[tid] = a.k_scales[at + tid];
+        else vs_s[tid - AM_KEYS] = a.v_scales[at + tid - AM_KEYS];
+        __syncthreads();
+        // ---- scores of rows 4 rg .. + 3, keys kg + 16 j ----
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+        const float* qr = q_s + rg * 4 * hd;
+        const __half* kr = k_s + kg * hs;
+#pragma unroll 2
+        for (int d = 0; d < hd; d += 4) {
+            float4 q4[4], k4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q4[i] = *reinterpret_cast<const float4*>(qr + i * hd + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k4[j] = am_floats(kr + 16 * j * hs + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[i][j] = fmaf(q4[i].x, k4[j].x, s[i][j]); s[i][j] = fmaf(q4[i].y, k4[j].y, s[i][j]);
+                    s[i][j] = fmaf(q4[i].z, k4[j].z, s[i][j]); s[i][j] = fmaf(q4[i].w, k4[j].w, s[i][j]);
+                }
+        }
+        // ---- their weights ----
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float top = AQ_NEG;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = kg + 16 * j, p = j0 + key;
+                const bool seen = p >= max(lo_w[i], lo) && p < min(hi_w[i], hi);
+                s[i][j] = seen ? s[i][j] * ks_s[key] : AQ_NEG;
+                top = fmaxf(top, s[i][j]);
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(m_r[i], top);
+            const float m_use = top == AQ_NEG ? 0.0f : top, f = expf(m_r[i] - m_use);
+            m_r[i] = top;
+            l_r[i] *= f;
+#pragma unroll
+            for (int d = 0; d < 4 * NJ; ++d) acc[i][d] *= f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = kg + 16 * j, p = j0 + key;
+                const bool seen = p >= max(lo_w[i], lo) && p < min(hi_w[i], hi);
+                const float w = expf(s[i][j] - m_use);
+                l_r[i] += w;
+                s[i][j] = seen ? w * vs_s[key] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p_s[rg * AM_KEYS + kg + 16 * j] = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+        __syncwarp();
+        // ---- outputs: dimensions 4 kg + 64 j ----
+#pragma unroll 4
+        for (int key = 0; key < AM_KEYS; ++key) {
+            const float4 w = p_s[rg * AM_KEYS + key];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                if (64 * j + 64 <= hd || 64 * j + 4 * kg < hd) {
+                    const float4 v = am_floats(v_s + key * hd + 64 * j + 4 * kg);
+                    const float we[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[i][4 * j] = fmaf(we[i], v.x, acc[i][4 * j]);
+                        acc[i][4 * j + 1] = fmaf(we[i], v.y, acc[i][4 * j + 1]);
+                        acc[i][4 * j + 2] = fmaf(we[i], v.z, acc[i][4 * j + 2]);
+                        acc[i][4 * j + 3] = fmaf(we[i], v.w, acc[i][4 * j + 3]);
+                    }
+                }
+        }
+        __syncwarp();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float l = l_r[i];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const int r = rg * 4 + i;
+        if (r >= rows) continue;
+        const size_t th = place_s[r];
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        float* p = a.n_splits > 1 ? a.partial + (th * a.n_splits + split) * (hd + 2) : nullptr;
+        if (p != nullptr && kg == 0) {
+            // base-2 units, as the kernel of few rows leaves them
+            p[0] = l != l ? INFINITY : m_r[i] * 1.4426950408889634f;
+            p[1] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int d = 64 * j + 4 * kg;
+            if (d >= hd) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (p != nullptr) p[2 + d + e] = acc[i][4 * j + e];
+                else ((T*)a.out)[th * hd + d + e] = from_f32<T>(acc[i][4 * j + e] * inv);
+            }
         }
     }
 }
@@ -955,7 +1166,7 @@ __global__ void attention_q8_merge_kernel(AttnQ8Args a) {
     for (int b = threadIdx.x; b < a.n_rows; b += blockDim.x) {
         const int from = a.cu_seqlens[b], to = a.cu_seqlens[b + 1];
         if (from >= 0 && from <= token && token < to && to <= a.n_tokens)
-            held |= (long long)(token - from) * G + head % G < (long long)a.q_groups * AG_ROWS;
+            held |= (long long)(token - from) * G + head % G < (long long)a.q_groups * a.block_rows;
     }
     if (!__syncthreads_or(held)) return;
     const float* p = a.partial + th * n_splits * (hd + 2);
@@ -991,9 +1202,8 @@ static constexpr int aq_blocks_an_sm(int hd, int rows) {
     return hd == 128 ? (rows == 16 ? 3 : 2) : (rows <= 16 ? 4 : 3);
 }
 
-// matrix rows a block takes, from the most tokens a row brings
-static int aq_block_rows(int max_row_tokens, int group, int hd, int dtype) {
-    if (!aq_on_tensor_cores(hd, dtype)) return AG_ROWS;
+// matrix rows a block of the tensor-core kernel takes, from the most tokens a row brings
+static int aq_block_rows(int max_row_tokens, int group) {
     const long long tiles = ((long long)max_row_tokens * group + 7) / 8;
     if (tiles <= 4) return (int)tiles * 8;
     const long long blocks = (tiles + 3) / 4;
@@ -1011,18 +1221,25 @@ struct AqPlan {
 static AqPlan aq_plan(int n_tokens, int n_rows, int max_row_tokens, int span, int n_heads, int n_kv, int hd, int dtype) {
     AqPlan p{};
     const int group = n_heads / n_kv;
-    p.rows = aq_block_rows(max_row_tokens, group, hd, dtype);
-    const long long groups = ((long long)max_row_tokens * group + p.rows - 1) / p.rows;
-    const long long items = (long long)n_rows * n_kv * groups;
     const int pages = span <= 0 ? 1 : (span + MF_PAGE - 1) / MF_PAGE, sms = mf_sm_count();
-    if (!aq_on_tensor_cores(hd, dtype)) {
-        long long splits = 3LL * sms / items;
+    const bool tensor = aq_on_tensor_cores(hd, dtype);
+    auto items_of = [&](int rows) { return (long long)n_rows * n_kv * (((long long)max_row_tokens * group + rows - 1) / rows); };
+    if (!tensor) {
+        // 32 rows a block where that many are worth it and its pages are two blocks an SM at least.  us, 8 rows a block /
+        // 32 (40 heads, 8 of keys, 128): 16 sequences of 3 tokens behind 2,000 346 / 244, 4 of 2 behind 600 31 / 33;
+        // 38 of 36 behind 75 to 151 334 / 319; 4 of 1 to 3 behind 60 to 611 (14 and 2 heads of 64) 14.4 / 20.5; one of 512
+        // behind none (28 and 4 of 128) 191 / 162; 8 of 16 behind 1,000 (8 and 2 of 256) 123 / 88; 39 of 8 behind 340 to
+        // 680 (16 and 4 of 128) 145 / 160, the one loss found.
+        p.rows = (long long)max_row_tokens * group > AM_LEAST && items_of(AM_ROWS) * pages >= 2LL * sms ? AM_ROWS : AG_ROWS;
+        long long splits = 3LL * sms / items_of(p.rows);
         if (splits > pages) splits = pages;
         if (splits > AQ_MAX_SPLITS) splits = AQ_MAX_SPLITS;
         p.splits = splits < 1 ? 1 : (int)splits;
         p.floats = p.splits > 1 ? (long long)n_tokens * n_heads * p.splits * (hd + 2) : 0;
         return p;
     }
+    p.rows = aq_block_rows(max_row_tokens, group);
+    const long long items = items_of(p.rows);
     const int held = sms * aq_blocks_an_sm(hd, p.rows);
     int cluster = 1;
     while (2 * cluster <= AQ_CLUSTER && 2 * cluster * items <= held && 2 * cluster <= (pages + 3) / 4) cluster *= 2;
@@ -1082,9 +1299,10 @@ static int launch_mma(const AttnQ8Args& a, int items, int splits, cudaStream_t s
            : splits == 1 ? launch_mma_as<HD, FMT, NT, KT, AQ_WHOLE, STAGES, minb>(a, items, 0, stream)
                          : launch_mma_as<HD, FMT, NT, KT, AQ_SPLIT, STAGES, minb>(a, items, 0, stream);
 }
+static unsigned ag_by_row(int hd) { return (unsigned)((0x100000000ULL + hd / 4 - 1) / (hd / 4)); }
 template <typename T, int FMT, int ND> static int launch_generic_as(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
-    const int smem = (AG_KEYS * (2 * a.hd + 1) + AG_ROWS * a.hd + 2 * AG_KEYS + AG_ROWS * AG_KEYS) * 4;
-    constexpr int hd = 32 * ND, most = (AG_KEYS * (2 * hd + 1) + AG_ROWS * hd + 2 * AG_KEYS + AG_ROWS * AG_KEYS) * 4;
+    const int smem = (AG_KEYS * (2 * a.hd + 4) + AG_ROWS * a.hd + 2 * AG_KEYS + AG_ROWS * AG_KEYS) * 4;
+    constexpr int hd = 32 * ND, most = (AG_KEYS * (2 * hd + 4) + AG_ROWS * hd + 2 * AG_KEYS + AG_ROWS * AG_KEYS) * 4;
     static bool opened[AQ_MAX_DEVICES] = {};
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
@@ -1094,10 +1312,29 @@ template <typename T, int FMT, int ND> static int launch_generic_as(const AttnQ8
             return (int)e;
         if (dev >= 0 && dev < AQ_MAX_DEVICES) opened[dev] = true;
     }
-    mf_launch(attention_q8_generic_kernel<T, FMT, ND>, grid, dim3(AG_WARPS * 32), smem, stream, a);
+    mf_launch(attention_q8_generic_kernel<T, FMT, ND>, grid, dim3(AG_WARPS * 32), smem, stream, a, ag_by_row(a.hd));
+    return MF_LAUNCH_CHECK();
+}
+template <typename T, int FMT, int NJ> static int launch_rows_as(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
+    auto bytes = [](int hd) { return AM_KEYS * (2 * hd + 4) * 2 + (AM_ROWS * hd + 2 * AM_KEYS + AM_ROWS * AM_KEYS) * 4; };
+    static bool opened[AQ_MAX_DEVICES] = {};
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
+    if (dev < 0 || dev >= AQ_MAX_DEVICES || !opened[dev]) {
+        if (cudaError_t e = cudaFuncSetAttribute(attention_q8_rows_kernel<T, FMT, NJ>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(64 * NJ)))
+            return (int)e;
+        if (dev >= 0 && dev < AQ_MAX_DEVICES) opened[dev] = true;
+    }
+    mf_launch(attention_q8_rows_kernel<T, FMT, NJ>, grid, dim3(128), (size_t)bytes(a.hd), stream, a, ag_by_row(a.hd));
     return MF_LAUNCH_CHECK();
 }
 template <typename T, int FMT> static int launch_generic(const AttnQ8Args& a, dim3 grid, cudaStream_t stream) {
+    if (a.block_rows == AM_ROWS)
+        return a.hd <= 64    ? launch_rows_as<T, FMT, 1>(a, grid, stream)
+               : a.hd <= 128 ? launch_rows_as<T, FMT, 2>(a, grid, stream)
+               : a.hd <= 192 ? launch_rows_as<T, FMT, 3>(a, grid, stream)
+                             : launch_rows_as<T, FMT, 4>(a, grid, stream);
     return a.hd <= 32   ? launch_generic_as<T, FMT, 1>(a, grid, stream)
            : a.hd <= 64 ? launch_generic_as<T, FMT, 2>(a, grid, stream)
            : a.hd <= 128 ? launch_generic_as<T, FMT, 4>(a, grid, stream)
@@ -1143,6 +1380,7 @@ extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v
     const long long groups = ((long long)max_row_tokens * (n_heads / n_kv) + plan.rows - 1) / plan.rows;
     if (groups * n_kv > 32767) return MF_ERR_UNSUPPORTED;
     a.q_groups = (int)groups;
+    a.block_rows = plan.rows;
     a.max_end = ring > 0 ? 1 << 30 : table_stride * MF_PAGE;
     // (the pages of all items are counted in 32 bits)
     const long long row_pages = ring > 0 ? ((long long)window + n_tokens) / MF_PAGE + 3 : table_stride;

@@ -148,7 +148,7 @@ class Engine:
                 if name not in libs:
                     libs.append(name)
         if self.cache_dtype is not None:
-            libs += ["cache_q8", "attention_q8"]
+            libs += ["cache_q8", "attention_q8", "attention_q8_tc"]
         build.prebuild(libs)
         # one word for the error bits of this engine's kernels, read back without waiting: after
         # every step it is copied to pinned host memory, and the next step (or check_status)

@@ -308,6 +308,37 @@ def test_offsets_beyond_32_bits(dtype, dim):
 
 
 @FORMATS
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 16), (torch.float32, 64), (torch.float32, 112), (torch.float32, 128),
+                                       (torch.float32, 192), (torch.float32, 256), (torch.bfloat16, 96)])
+@pytest.mark.parametrize("rows,heads,kv,window", [
+    ([(4, 300), (3, 261), (1, 310), (0, 5), (4, 0), (4, 60), (2, 255), (4, 256)], 40, 8, 0), ([(10, 4990), (7, 13)], 4, 2, 0),
+    ([(40, 290)] * 4, 12, 12, 130), ([(4, 600)] * 16, 20, 4, 200)], ids=str)
+def test_attention_of_many_rows_on_the_fp32_pipe(rows, heads, kv, window, dtype, dim, fmt):
+    new, past = zip(*rows)
+    ends, cu = [n + p for n, p in zip(new, past)], [0] + np.cumsum(new).tolist()
+    ring = -(-(window + max(new) - 1) // PAGE) * PAGE if window else 0
+    gen, rng = torch.Generator().manual_seed(dim), np.random.RandomState(6)
+    table, n_pages = make_table(ends, ring, rng)
+    pages = make_pages(table, n_pages, ends, ring, kv, dim, fmt, gen)
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(dtype).to(DEV)
+    # what decides that a block takes 32 rows
+    span = max(ends) if not window else min(max(ends), window + max(new) + PAGE - 1)
+    blocks = len(rows) * kv * -(-max(new) * (heads // kv) // 32)
+    assert max(new) * (heads // kv) > 12 and blocks * -(-span // PAGE) >= 2 * K.sm_count(q.device)
+    got = run_attention(q, pages, cu, ends, table, ring, heads, kv, dim, window, dim ** -0.5)
+    want, *sizes = plain.attention(q, pages, cu, ends, table, ring, heads, kv, window, dim ** -0.5)
+    tol = plain.attention_tolerance(want, *sizes, dtype, dim, fmt)
+    assert ((got.double().cpu() - want).abs() <= tol).all()
+    # a value of NaN at the first row's last position but one: the last two tokens of its head group see it
+    place = (ends[0] - 2) % ring if ring else ends[0] - 2
+    pages.v_scale[table[0][place // PAGE], 0, place % PAGE] = float("nan")
+    again = run_attention(q, pages, cu, ends, table, ring, heads, kv, dim, window, dim ** -0.5)
+    hit = torch.zeros(cu[-1], heads, dtype=torch.bool, device=DEV)
+    hit[new[0] - 2:new[0], :heads // kv] = True
+    assert torch.isnan(again[hit]).all() and torch.equal(again[~hit], got[~hit])
+
+
+@FORMATS
 @pytest.mark.parametrize("heads,kv,dim", [(6, 2, 128), (5, 1, 64)])
 @pytest.mark.parametrize("rows,window,spread", [
     ([(300, 1000)], 0, 0.0), ([(1, 5), (257, 0), (128, 4000), (129, 127), (2, 0)], 0, 8.0), ([(64, 64)] * 5, 0, 0.0),
