@@ -96,12 +96,11 @@ __device__ __forceinline__ float lds32(uint32_t at) {
 // 2^10: nothing is near overflow until then, and the usual step needs one vote and no exchange between
 // lanes.
 //
-// Bound by bytes where rows are few and caches long: 64 sequences of 4,097 to 8,192 positions, one token each, 28
-// heads, 4 of keys, 128: 65 us, 5.3 TB/s (0.81 of a copy), two thirds of that the 61 us of one launch whose
-// blocks wait for their first pages 3 us.  Where rows are many, a step of 16 keys takes a warp about 1,650 clocks
-// at 24 rows (16 sequences with 4 drafts each over 2,000 positions: 30.8 us): its loads, conversions, products and
+// Bound by bytes where rows are few and caches long: 64 sequences of 2,047 to 8,100 positions, one token each, 28
+// heads, 4 of keys, 128: 65 us, 5.3 TB/s (0.81 of a copy), the first pages' latency and the join included.  Where rows are many, a step of 16 keys takes a warp about 1,650 clocks
+// at 24 rows (16 sequences with 4 drafts each over 1,501 to 3,001 positions: 30.8 us): its loads, conversions, products and
 // exponentials follow one another, and two or three warps a scheduler do not hide them all.  Short calls are
-// latency (8 sequences of 500 to 2,048 positions: 10.3 us).
+// latency (8 sequences of 1,801 to 2,047 positions: 10.3 us).
 //
 // Layouts: row r of a score tile is key 4 (r' >> 1) + 2 (r >> 3) + (r & 1), r' = r & 7, of the step's 16, so that
 // the keys a thread multiplies values of are the four from 4 t on.  Both operands of a score see the same

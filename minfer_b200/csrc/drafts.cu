@@ -20,9 +20,9 @@
 // in registers between the two.  The second joins the pieces, decides (every block of a sequence finds the
 // same) and passes over the one row that the token comes from: a warp takes steps of 128 tokens and leaves
 // their sums.  The third finds the step that holds the answer and goes through it again.  (The second and
-// third as one, a cluster of eight blocks a sequence: 21 us for one sequence with four drafts over 152,064
+// third as one, a cluster of eight blocks a sequence: 21 us for one sequence with four drafts over 151,936
 // tokens where this takes 14, since eight SMs form 300,000 exponentials in double; 70 us for 64 of them
-// where this takes 57.)  Of those 57 us the first launch is some 33, 5.9 TB/s of its 195 MB; the second forms
+// where this takes 57.)  Of those 57 us the first launch is some 33, 5.9 TB/s of its 190 MB; the second forms
 // ten million exponentials in double, twenty instructions each, and is bound by their latency and issue: 20 us
 // with the 32 warps an SM that 64 registers leave room for and two steps in flight, 24 with 16 warps and four.
 // Where the drafts have distributions of their own, all rows' exponentials are double: 129 us of 64 sequences.
