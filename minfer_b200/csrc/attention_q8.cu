@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
     const int G = a.n_heads / a.n_kv;
 
     // ---- which pages of which items ----
-    int b = blockIdx.z, item = blockIdx.y, page0 = 0, page1 = 0;          // pages [page0, page1) of the item
+    int b = blockIdx.z, item = MODE == AQ_WHOLE ? blockIdx.x : blockIdx.y, page0 = 0, page1 = 0;          // pages [page0, page1) of the item
     int todo = 0;                                                         // AQ_SHARED: pages left to this block
     AqFirst first_of;
     AqRow row;
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
         // (uniform over a cluster)
         if (item >= row.items) { pdl_wait(); return; }
         const int chunk = MODE == AQ_SPLIT ? (row.pages + a.n_splits - 1) / a.n_splits : row.pages;
-        page0 = min(row.pages, (int)blockIdx.x * chunk);
+        page0 = MODE == AQ_SPLIT ? min(row.pages, (int)blockIdx.x * chunk) : 0;
         page1 = min(row.pages, page0 + chunk);
     }
     bool waited = false;
@@ -864,7 +864,7 @@ __global__ void __launch_bounds__(AG_WARPS * 32) attention_q8_generic_kernel(Att
     float* vs_s = ks_s + AG_KEYS;
     float* p_s = vs_s + AG_KEYS;                           // [AG_ROWS][AG_KEYS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x, hk = blockIdx.y / a.q_groups, qg = blockIdx.y - hk * a.q_groups, b = blockIdx.z;
+    const int split = blockIdx.y, hk = blockIdx.x / a.q_groups, qg = blockIdx.x - hk * a.q_groups, b = blockIdx.z;
     const int G = a.n_heads / a.n_kv;
     int tok0, count, end;
     aq_bounds(a, b, &tok0, &count, &end);
@@ -1009,7 +1009,7 @@ __global__ void __launch_bounds__(128) attention_q8_rows_kernel(AttnQ8Args a, un
     float4* p_s = (float4*)(vs_s + AM_KEYS);               // [8][AM_KEYS]: the weights of four rows
     __shared__ size_t place_s[AM_ROWS];
     const int tid = threadIdx.x, rg = tid >> 4, kg = tid & 15;
-    const int split = blockIdx.x, hk = blockIdx.y / a.q_groups, qg = blockIdx.y - hk * a.q_groups, b = blockIdx.z;
+    const int split = blockIdx.y, hk = blockIdx.x / a.q_groups, qg = blockIdx.x - hk * a.q_groups, b = blockIdx.z;
     const int G = a.n_heads / a.n_kv;
     int tok0, count, end;
     aq_bounds(a, b, &tok0, &count, &end);
@@ -1268,7 +1268,7 @@ static int launch_mma_as(const AttnQ8Args& a, int items, int blocks, cudaStream_
         if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return (int)e;
         if (dev >= 0 && dev < AQ_MAX_DEVICES) opened[dev] = true;
     }
-    const dim3 grid = MODE == AQ_SHARED ? dim3(blocks) : dim3(a.n_splits, items, a.n_rows);
+    const dim3 grid = MODE == AQ_SHARED ? dim3(blocks) : MODE == AQ_WHOLE ? dim3(items, 1, a.n_rows) : dim3(a.n_splits, items, a.n_rows);
     if (MODE != AQ_SPLIT) {
         mf_launch(kernel, grid, dim3(AQ_WARPS * 32), smem, stream, a);
         if (int e = MF_LAUNCH_CHECK()) return e;
@@ -1377,7 +1377,7 @@ extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v
     a.n_tokens = n_tokens; a.n_rows = n_rows; a.n_heads = n_heads; a.n_kv = n_kv; a.hd = hd; a.window = window;
     a.n_splits = plan.splits < 0 ? 1 : plan.splits; a.scale = scale; a.status = status;
     const long long groups = ((long long)max_row_tokens * (n_heads / n_kv) + plan.rows - 1) / plan.rows;
-    if (groups * n_kv > 32767) return MF_ERR_UNSUPPORTED;
+    if (groups * n_kv > 0x7fffffffLL) return MF_ERR_UNSUPPORTED;
     a.q_groups = (int)groups;
     a.block_rows = plan.rows;
     a.max_end = ring > 0 ? 1 << 30 : table_stride * MF_PAGE;
@@ -1385,7 +1385,7 @@ extern "C" int mf_attention_q8(const void* q, const void* k_codes, const void* v
     const long long row_pages = ring > 0 ? ((long long)window + n_tokens) / MF_PAGE + 3 : table_stride;
     if (plan.splits < 0 && row_pages * groups * n_kv * n_rows > 0x7fffffffLL) plan.splits = 1;
     const int items = (int)(groups * n_kv), n_splits = a.n_splits;
-    const dim3 grid(n_splits, items, n_rows);
+    const dim3 grid(items, n_splits, n_rows);
     int e;
     if (aq_on_tensor_cores(hd, dtype)) {
 #define AQ_GO(HD, NT, KT, STAGES)                                                                 \

@@ -1328,7 +1328,8 @@ def attention_paged_q8(q: torch.Tensor, pages: Q8Pages, cu_seqlens: torch.Tensor
     cu_seqlens[b+1]-1`` of ``q`` [tokens, n_heads, head_dim] at positions ``seq_end[b] - count .. seq_end[b] - 1``,
     and the pages hold every position up to there, the step's own included.  A token sees the positions up
     to its own (the last ``window`` of them where that is not 0) and reads zeros if there is none.
-    ``max_row_tokens``: the most tokens a row brings; ``max_end``: a bound of ``seq_end`` (it sizes the splits).
+    ``max_row_tokens``: the most tokens a row brings; ``max_end``: a bound of ``seq_end`` (it sizes the
+    splits, and what of a long portion's pages is unpacked: a longer row then sets status bit 2).
     A page that a token would see and its row has not sets status bit 2; what such a row reads is undefined, but
     nothing outside the pages is touched and other rows are not.  Portions of many tokens run
     on tcgen05 (``q8_on_tcgen05``), keys and values rounded to halves, over scratch of at most ``Q8_PORTION_BYTES``

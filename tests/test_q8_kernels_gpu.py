@@ -363,6 +363,119 @@ def test_portions_on_tcgen05(rows, window, spread, heads, kv, dim, fmt, monkeypa
         assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 16), (torch.bfloat16, 64)])
+def test_more_blocks_than_a_grid_has_rows(dtype, dim, monkeypatch):
+    """A long portion of very many heads: items beyond 65,535."""
+    monkeypatch.setattr(K, "q8_on_tcgen05", lambda *a: False)
+    heads, n, fmt = 1040, 2050, torch.int8
+    gen, rng = torch.Generator().manual_seed(1), np.random.RandomState(2)
+    table, n_pages = make_table([n], 0, rng)
+    pages = make_pages(table, n_pages, [n], 0, heads, dim, fmt, gen, junk=False)
+    q = torch.randn(n, heads, dim, generator=gen).to(dtype).to(DEV)
+    got = run_attention(q, pages, [0, n], [n], table, 0, heads, heads, dim, 0, 0.2)
+    order = ints(table[0]).long()
+    sees = torch.ones(n, n, dtype=torch.bool, device=DEV).tril()
+    for h in (0, 517, 1039):
+        k, v = ((c[order, h].double() * s[order, h].double().unsqueeze(-1)).reshape(-1, dim)[:n]
+                for c, s in ((pages.k, pages.k_scale), (pages.v, pages.v_scale)))
+        s = (q[:, h].double() @ k.T * 0.2).masked_fill(~sees, -np.inf)
+        p = torch.softmax(s, -1)
+        size = (q[:, h].double().abs() @ k.abs().T * 0.2).masked_fill(~sees, 0.0).amax(-1)
+        top = (p * pages.v_scale[order, h].double().reshape(-1)[:n]).amax(-1)
+        keys = torch.arange(1, n + 1, device=DEV).double()
+        want, mass = p @ v, p @ v.abs()
+        tol = plain.attention_tolerance(want.unsqueeze(1), mass.unsqueeze(1), top.unsqueeze(1), size.unsqueeze(1), keys,
+                                        dtype, dim, fmt)
+        assert ((got[:, h].double() - want).abs() <= tol[:, 0]).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [0, 70, 500])
+def test_lengths_and_offsets_that_are_anything_on_tcgen05(window, dim, monkeypatch):
+    monkeypatch.setattr(K, "q8_on_tcgen05", lambda *a: True)
+    heads, kv, fmt, big, longest = 4, 2, torch.int8, 2 ** 31 - 1, 4000
+    gen, rng = torch.Generator().manual_seed(1), np.random.RandomState(2)
+    ends, new = [longest, 90, 180, 650, 33, 320], [40, 3, 130, 40, 1, 300]
+    cu = [0] + np.cumsum(new).tolist()
+    table, n_pages = make_table(ends, 0, rng)
+    pages = make_pages(table, n_pages, ends, 0, kv, dim, fmt, gen)
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(torch.bfloat16).to(DEV)
+    want, *sizes = plain.attention(q, pages, cu, ends, table, 0, heads, kv, window, 0.2)
+    most = float(pages.v_scale.nan_to_num(0.0).max()) * plain.LIMIT[fmt]
+    tol = plain.halves_tolerance(want, *sizes, most)
+
+    def call(cu, ends, most_new=300):
+        out, st = torch.full_like(q, 7.0), status_word()
+        K.attention_paged_q8(q, pages, ints(cu), ints(ends), ints(table), len(table[0]), 0, out, most_new, longest, heads,
+                             kv, dim, window, 0.2, st)
+        return out, (out.double().cpu() - want).abs() <= tol, int(st.item())
+
+    def rows(x, which):
+        return torch.cat([x[cu[b]:cu[b + 1]] for b in which])
+    out, right, st = call(cu, ends)
+    assert st == 0 and right.all()
+    for wild in (big, big - 31, 2 ** 30, longest + 1):
+        out, right, st = call(cu, [ends[0], wild, ends[2], wild, ends[4], ends[5]])
+        assert st == 2 and rows(right, [0, 2, 4, 5]).all()
+    for wild in (-1, -2 ** 31, -2 ** 31 + 40):
+        out, right, st = call(cu, [ends[0], wild, ends[2], wild, ends[4], ends[5]])
+        assert st == 0 and rows(right, [0, 2, 4, 5]).all() and (rows(out, [1, 3]) == 0).all()
+    for wild in (-1, -2 ** 31, cu[-1] + 1, big):
+        broken = list(cu)
+        broken[2] = wild
+        out, right, st = call(broken, ends)
+        assert st == 0 and rows(right, [0, 3, 4, 5]).all() and (rows(out, [1, 2]) == 7.0).all()
+    # a row that brings more tokens than was said, and pages that are not there
+    out, right, st = call(cu, ends, most_new=64)
+    assert rows(right, [0, 1, 3, 4]).all()
+    for bad in (-1, n_pages, big):
+        broken = [list(r) for r in table]
+        broken[0][-1] = broken[2][0] = bad
+        out, st = torch.full_like(q, 7.0), status_word()
+        K.attention_paged_q8(q, pages, ints(cu), ints(ends), ints(broken), len(table[0]), 0, out, 300, longest, heads, kv,
+                             dim, window, 0.2, st)
+        assert int(st.item()) == 2
+        assert rows((out.double().cpu() - want).abs() <= tol, [1, 3, 4, 5]).all() and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("heads", [6, 40])
+def test_portions_captured_twice_and_on_another_stream(heads, monkeypatch):
+    monkeypatch.setattr(K, "q8_on_tcgen05", lambda *a: True)
+    kv, dim, fmt = 2, 128, torch.float8_e4m3fn
+    gen, rng = torch.Generator().manual_seed(1), np.random.RandomState(2)
+    ends, cu = [1500, 900, 64], [0, 300, 333, 397]
+    table, n_pages = make_table(ends, 0, rng)
+    pages = make_pages(table, n_pages, ends, 0, kv, dim, fmt, gen)
+    qs = [torch.randn(cu[-1], heads, dim, generator=gen).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    eager = [run_attention(q, pages, cu, ends, table, 0, heads, kv, dim, 0, 0.1) for q in qs]
+    cu_d, end_d, table_d, st = ints(cu), ints(ends), ints(table), status_word()
+    torch.cuda.synchronize()
+
+    def call(q, out):
+        K.attention_paged_q8(q, pages, cu_d, end_d, table_d, len(table[0]), 0, out, 300, 1500, heads, kv, dim, 0, 0.1, st)
+    outs, graphs = [], []
+    for q in qs:
+        out, graph = torch.zeros_like(q), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            call(q, out)
+        outs.append(out)
+        graphs.append(graph)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+    # two calls at once
+    sides, outs = [torch.cuda.Stream() for _ in qs], [torch.zeros_like(q) for q in qs]
+    for side, q, out in zip(sides, qs, outs):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(3):
+                call(q, out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, eager)) and int(st.item()) == 0
+
+
 @pytest.mark.parametrize("window", [0, 90])
 @pytest.mark.parametrize("back", [True, False])
 def test_a_page_table_wider_than_its_rows(window, back, monkeypatch):
