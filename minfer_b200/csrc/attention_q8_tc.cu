@@ -4,11 +4,12 @@
 //   o_i = sum_j p_ij vs_j vc_j / sum_j p_ij,   p_ij = exp(scale q_i . kc_j ks_j - max)
 //
 // Keys and values go to the tensor cores as halves, each brought below 2^15 by one power of two of its 128
-// positions (a half has eight times a bfloat16's precision, and scales of neighbouring positions would have to
-// be 2^20 apart to reach the numbers below its normal range); queries are exact halves by a power of two of
-// their vector, and so are probabilities rounded: each of the three is off by 2^-11.  (Codes multiplied as they
-// are, exactly, with the scales applied to scores and probabilities: a row's 128 keys need 384 scales out of
-// shared memory, 3,072 of the 5,200 cycles that a tile then took; this way it takes 3,000.)
+// positions; queries are exact halves by a power of two of their vector; probabilities are rounded to halves, too:
+// keys, values and probabilities are off by 2^-11 each, where bfloat16 is by 2^-8.  (Codes multiplied as they are,
+// exactly, with the scales applied to scores and probabilities: a row's 128 keys need 384 scales out of shared
+// memory, 3,072 of the 5,200 clocks that a tile then took; this way it takes 3,800.)  Where scales of 128 positions
+// are more than 2^QT_APART apart (a half's range; a token may not see the one that is far above the others), every
+// position has a power of two of its own, which its scores and probabilities are multiplied by.
 //
 // Three launches:
 //   unpack   what the rows' tokens can see, position behind position (a window over a ring becomes a
@@ -30,6 +31,8 @@
 #include "prefill_tc.cuh"
 #include "q8.cuh"
 
+#include <type_traits>
+
 #define QT_Q 128              // queries a tile
 #define QT_ITEM 256           // queries an item: two tiles
 #define QT_KEYS 128           // keys a tile
@@ -37,6 +40,8 @@
 #define QT_BELOW 6.0f         // the reference is put 2^6 below the largest weight, and moves when one passes it by 2^14
 #define QT_ROOM 14.0f
 #define QT_LEAST 4            // least tiles a block takes
+#define QT_APART 16           // binary orders that scales of a tile share a power of two over
+#define QT_WIDE 1000.0f       // in place of a tile's exponents: its positions have their own
 #define QT_LEAST_VALUE (-60)  // values' power of two at least (sums of 2^(s_j - m) stay in float32's range)
 
 struct QtArgs {
@@ -58,7 +63,8 @@ struct QtArgs {
     // scratch
     __half* k16;              // [rows][n_kv][stretch][HD]
     __half* v16;
-    float2* powers;           // [rows][n_kv][stretch / 128]: the keys' power of two, the values' exponent
+    float2* powers;           // [rows][n_kv][stretch / 128]: the exponents of keys and values, or QT_WIDE
+    float* own;               // [rows][n_kv][stretch / 128][2][128]: the positions' powers of two, keys and values
     __half* q16;              // [tokens][n_heads][HD]
     float* factor;            // [tokens][n_heads]: scores in powers of two of 2
     int4* first;              // [blocks]: row, item of the row, tile of it, tiles a block
@@ -176,7 +182,7 @@ __global__ void __launch_bounds__(QU_THREADS) q8_unpack_kernel(QtArgs a, int n_t
         from[h] = there ? ((long long)page * a.n_kv + hk) * MF_PAGE : -1;
     }
     __shared__ float scale_s[QT_KEYS];
-    __shared__ unsigned most_s[QT_KEYS / 32];
+    __shared__ unsigned most_s[QT_KEYS / 32], least_s[QT_KEYS / 32];
     pdl_wait();
     const uint8_t* codes = is_v ? a.v_codes : a.k_codes;
     constexpr int EACH = QT_KEYS * HD / 8 / QU_THREADS;
@@ -197,24 +203,34 @@ __global__ void __launch_bounds__(QU_THREADS) q8_unpack_kernel(QtArgs a, int n_t
         if (is_v && vs != vs) x = 0.0f;
         if (!is_v && vs != vs) x = vs;
         scale_s[tid] = x;
-        const unsigned most = __reduce_max_sync(0xffffffffu, x == x ? __float_as_uint(fabsf(x)) : 0u);
-        if ((tid & 31) == 0) most_s[tid >> 5] = most;
+        const unsigned bits = x == x ? __float_as_uint(fabsf(x)) : 0u;
+        const unsigned most = __reduce_max_sync(0xffffffffu, bits);
+        const unsigned least = __reduce_min_sync(0xffffffffu, bits == 0 ? 0x7f800000u : bits);
+        if ((tid & 31) == 0) { most_s[tid >> 5] = most; least_s[tid >> 5] = least; }
     }
     __syncthreads();
-    // the largest scale to 2^5 .. 2^6, times a code below 2^15
+    // the largest scale (or every one) to 2^5 .. 2^6, times a code below 2^15
+    auto power_of = [&](unsigned bits) {
+        return bits == 0 ? 0 : min(max((int)(bits >> 23) - 127 - 5, is_v ? QT_LEAST_VALUE : -120), 120);
+    };
     const unsigned most = max(max(most_s[0], most_s[1]), max(most_s[2], most_s[3]));
-    const int power = most == 0 ? 0 : min(max((int)(most >> 23) - 127 - 5, is_v ? QT_LEAST_VALUE : -120), 120);
-    const float down = __int_as_float((127 - power) << 23);
+    const unsigned least = min(min(least_s[0], least_s[1]), min(least_s[2], least_s[3]));
+    const int power = power_of(most);
+    const bool wide = power - power_of(min(least, most)) > QT_APART;
     const long long tile = ((long long)b * a.n_kv + hk) * tiles + i;
-    if (tid == 0) {
-        if (is_v) a.powers[tile].y = (float)power;
-        else a.powers[tile].x = __int_as_float((127 + power) << 23);
+    if (tid == 0) (is_v ? a.powers[tile].y : a.powers[tile].x) = wide ? QT_WIDE : (float)power;
+    if (tid < QT_KEYS) {
+        const float x = scale_s[tid];
+        const int mine = wide ? power_of(x == x ? __float_as_uint(fabsf(x)) : 0u) : power;
+        a.own[tile * (2 * QT_KEYS) + (is_v ? QT_KEYS : 0) + tid] = __int_as_float((127 + mine) << 23);
+        scale_s[tid] = x * __int_as_float((127 - mine) << 23);
     }
+    __syncthreads();
     __half* out = (is_v ? a.v16 : a.k16) + tile * (QT_KEYS * HD);
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
         const int unit = tid + j * QU_THREADS;
-        const float by = scale_s[unit / (HD / 8)] * down;
+        const float by = scale_s[unit / (HD / 8)];
         float v[8];
         q8_floats<FMT>(w[j].x, v);
         q8_floats<FMT>(w[j].y, v + 4);
@@ -484,7 +500,7 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ---- softmax: four warps for each query tile, one thread a query row (two threads, which tell each other
-        // their halves' maxima, take 4,300 cycles a tile where this takes XXX) ----
+        // their halves' maxima, take 4,300 clocks a tile where this takes 3,800) ----
         const int t = (warp - 4) >> 2;
         const int quarter = warp & 3;                    // the 32 lanes of tensor memory this warp may touch
         const int trow = quarter * 32 + lane;            // row of the tile
@@ -503,12 +519,18 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const int start = at.row.end - at.row.count, wpos = start + q0t + quarter * 32;
             const bool real = qrow < at.row.count;
             const float by = real ? a.factor[(long long)(at.row.tok0 + qrow) * a.n_heads + at.head] : 1.0f;
-            float m = -INFINITY, l = 0.0f;
-            const float2* powers = a.powers + (at.b * a.n_kv + at.head / (a.n_heads / a.n_kv)) * (long long)(a.stretch / QT_KEYS) + at.lo + at.off;
-            float2 power = part_of ? powers[0] : make_float2(1.0f, 0.0f);
+            // the reference, the sum, and an exponent that outputs are to be multiplied by (0 unless scores are beyond
+            // 2^20, where a reference does not tell a value's exponent from a rounding)
+            float m = -INFINITY, l = 0.0f, r = 0.0f;
+            const long long tile0 = (at.b * a.n_kv + at.head / (a.n_heads / a.n_kv)) * (long long)(a.stretch / QT_KEYS) + at.lo + at.off;
+            const float2* powers = a.powers + tile0;
+            float2 power = part_of ? powers[0] : make_float2(0.0f, 0.0f);
             for (int j = 0; part_of && j < at.part; ++j) {
                 // (factors above 0 keep masked scores at -infinity)
-                const float by_tile = fminf(fmaxf(by * power.x, 1.2e-38f), 3e38f), values = power.y;
+                bool apart = power.x == QT_WIDE || power.y == QT_WIDE;
+                float by_tile = fminf(fmaxf(by * __int_as_float((127 + (int)power.x) << 23), 1.2e-38f), 3e38f), values = power.y;
+                if (apart) by_tile = 1.0f;
+                const float4* own = reinterpret_cast<const float4*>(a.own + (tile0 + j) * (2 * QT_KEYS));
                 if (j + 1 < at.part) power = powers[j + 1];
                 // S of this key tile is complete, and with it every earlier product of this query tile
                 if (!(ok = wait(&s_full[t], mine++))) break;
@@ -535,71 +557,118 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     mx2 = fa_max3(mx2, __uint_as_float(sr[e + 4]), __uint_as_float(sr[e + 5]));
                     mx3 = fa_max3(mx3, __uint_as_float(sr[e + 6]), __uint_as_float(sr[e + 7]));
                 }
-                const float m_tile = fmaf(fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)), by_tile, values);
-                const bool jump = m == -INFINITY ? m_tile > -INFINITY : m_tile - m > QT_ROOM;
-                const float m_new = jump ? m_tile - QT_BELOW : m;
+                float m_tile = fmaf(fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)), by_tile, values);
+                // (differences of scores beyond 2^20 are to be those of rounded products: a fused one is off by what the
+                // reference was rounded by)
+                apart = apart || (fabsf(m_tile) > 1048576.0f && m_tile > -INFINITY);
+                float r_new = r, m_far = -INFINITY;
+                if (apart) {
+                    // every position by its own powers of two; the largest weight: a score and its value's exponent
+                    float top = -INFINITY, v_top = -INFINITY;
+                    m_tile = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < QT_KEYS; e += 4) {
+                        const float4 k = own[e >> 2], v = own[(QT_KEYS + e) >> 2];
+                        const float ke[4] = {k.x, k.y, k.z, k.w}, ve[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const float x = __fmul_rn(__uint_as_float(sr[e + h]) * ke[h], by);
+                            const float power = (float)((__float_as_int(ve[h]) >> 23) - 127);
+                            sr[e + h] = __float_as_uint(x);
+                            top = fmaxf(top, x);
+                            if (x > -INFINITY) v_top = fmaxf(v_top, power);
+                            m_tile = fmaxf(m_tile, x + power);
+                        }
+                    }
+                    by_tile = 1.0f;
+                    values = 0.0f;
+                    if (fabsf(top) > 1048576.0f && top > -INFINITY) {
+                        const bool above = m == -INFINITY || top - m > 256.0f;      // (what came before weighs nothing)
+                        r_new = above ? v_top : fmaxf(r, v_top);
+                        m_far = above ? top : fmaxf(m, top);
+                    }
+                }
+                if (r != 0.0f && m_far == -INFINITY && m_tile - r - m > 256.0f) r_new = 0.0f;
+                const float m_here = m_tile - r_new;
+                const bool jump = m_far > -INFINITY ? m_far != m || r_new != r
+                                  : m == -INFINITY  ? m_here > -INFINITY
+                                                    : m_here - m > QT_ROOM;
+                const float m_new = !jump ? m : m_far > -INFINITY ? m_far : m_here - QT_BELOW;
                 const float m_off = m_new == -INFINITY ? 0.0f : m_new;
+                __syncwarp();
                 // the output so far is rescaled only if the reference moved for some row of this warp
                 if (j > 0 && __any_sync(0xffffffffu, jump)) {
-                    const float corr = jump ? (m == -INFINITY ? 0.0f : exp2f(m - m_off)) : 1.0f;
-                    l *= corr;
+                    const float corr = jump ? (m == -INFINITY ? 0.0f : exp2f((m - m_off) + (r - r_new))) : 1.0f;
+                    l *= jump ? (m == -INFINITY ? 0.0f : exp2f(m - m_off)) : 1.0f;
 #pragma unroll 1
                     for (int c0 = 0; c0 < HD; c0 += 32) {
-                        uint32_t r[32];
-                        fa_ld32(o_addr + (uint32_t)c0, r);
+                        uint32_t w[32];
+                        fa_ld32(o_addr + (uint32_t)c0, w);
                         fa_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
-                        fa_st32(o_addr + (uint32_t)c0, r);
+                        for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * corr);
+                        fa_st32(o_addr + (uint32_t)c0, w);
                     }
                 }
                 m = m_new;
+                r = r_new;
                 // weights 2^(s - m) times the values' power of two, their sum, and as halves into the first 64 columns
                 // of S
                 uint64_t l01 = 0, l23 = 0;               // four zeros
-                const uint64_t by2 = fa_pack2(by_tile, by_tile), off2 = fa_pack2(values - m_off, values - m_off);
+                const float off = apart ? -m_off : values - r - m_off;
+                const uint64_t by2 = fa_pack2(by_tile, by_tile), off2 = fa_pack2(off, off);
+                auto weigh = [&](auto apart_tag) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t pk[QT_KEYS / 4];
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t pk[QT_KEYS / 4];
 #pragma unroll
-                    for (int g = 0; g < QT_KEYS / 2; g += 4) {
-                        const int e = h * (QT_KEYS / 2) + g;
-                        float x0, x1, x2, x3;
-                        fa_unpack2(fa_fma2(qt_pair(sr + e), by2, off2), x0, x1);
-                        fa_unpack2(fa_fma2(qt_pair(sr + e + 2), by2, off2), x2, x3);
-                        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x0));
-                        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x1));
-                        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x2));
-                        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x3));
-                        l01 = fa_add2(l01, fa_pack2(x0, x1));
-                        l23 = fa_add2(l23, fa_pack2(x2, x3));
-                        pk[g >> 1] = qt_pack(x0, x1);
-                        pk[(g >> 1) + 1] = qt_pack(x2, x3);
+                        for (int g = 0; g < QT_KEYS / 2; g += 4) {
+                            const int e = h * (QT_KEYS / 2) + g;
+                            float x0, x1, x2, x3;
+                            fa_unpack2(fa_fma2(qt_pair(sr + e), by2, off2), x0, x1);
+                            fa_unpack2(fa_fma2(qt_pair(sr + e + 2), by2, off2), x2, x3);
+                            asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x0));
+                            asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x1));
+                            asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x2));
+                            asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x3));
+                            l01 = fa_add2(l01, fa_pack2(x0, x1));
+                            l23 = fa_add2(l23, fa_pack2(x2, x3));
+                            if constexpr (decltype(apart_tag)::value) {
+                                const float4 v = own[(QT_KEYS + e) >> 2];
+                                const float down_r = exp2f(-r);
+                                x0 *= apart ? v.x * down_r : 1.0f; x1 *= apart ? v.y * down_r : 1.0f;
+                                x2 *= apart ? v.z * down_r : 1.0f; x3 *= apart ? v.w * down_r : 1.0f;
+                            }
+                            pk[g >> 1] = qt_pack(x0, x1);
+                            pk[(g >> 1) + 1] = qt_pack(x2, x3);
+                        }
+                        fa_st32(s_addr + (uint32_t)(h * (QT_KEYS / 4)), pk);
+                        fa_wait_st();
+                        fa_fence_before();
+                        fa_arrive(fa_smem(h == 0 ? &p_half[t] : &p_full[t]));
                     }
-                    fa_st32(s_addr + (uint32_t)(h * (QT_KEYS / 4)), pk);
-                    fa_wait_st();
-                    fa_fence_before();
-                    fa_arrive(fa_smem(h == 0 ? &p_half[t] : &p_full[t]));
-                }
+                };
+                if (__any_sync(0xffffffffu, apart)) weigh(std::true_type{});
+                else weigh(std::false_type{});
                 float l0, l1, l2, l3;
                 fa_unpack2(l01, l0, l1);
                 fa_unpack2(l23, l2, l3);
-                l = fmaf((l0 + l1) + (l2 + l3), exp2f(-values), l);
+                l = fmaf((l0 + l1) + (l2 + l3), apart ? 1.0f : exp2f(r - values), l);
             }
             // ---- the item's result, or a part of it ----
             if (ok && part_of) {
                 if (!wait(&o_done[t], items++)) break;
                 fa_fence_after();
                 const bool whole = at.off == 0 && at.part == at.n;
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const float up_r = exp2f(r), inv = l == 0.0f ? 0.0f : up_r / l;
                 __nv_bfloat16* o = a.out + ((long long)(at.row.tok0 + qrow) * a.n_heads + at.head) * HD;
                 // (the first slot if another block began the item, else the second)
                 float* slot = a.slots + (2 * (size_t)blockIdx.x + (at.off > 0 ? 0 : 1)) * qt_slot_floats(HD);
                 const int irow = t * QT_Q + trow;
 #pragma unroll 1
                 for (int c0 = 0; c0 < HD; c0 += 32) {
-                    uint32_t r[32];
-                    fa_ld32(o_addr + (uint32_t)c0, r);
+                    uint32_t w[32];
+                    fa_ld32(o_addr + (uint32_t)c0, w);
                     fa_wait_ld();
                     if (whole && real) {
 #pragma unroll
@@ -607,8 +676,8 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                             uint32_t v[4];
 #pragma unroll
                             for (int h = 0; h < 4; ++h) {
-                                const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(r[e + 2 * h]) * inv,
-                                                                              __uint_as_float(r[e + 2 * h + 1]) * inv);
+                                const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(w[e + 2 * h]) * inv,
+                                                                              __uint_as_float(w[e + 2 * h + 1]) * inv);
                                 v[h] = *reinterpret_cast<const uint32_t*>(&x);
                             }
                             *reinterpret_cast<uint4*>(o + c0 + e) = make_uint4(v[0], v[1], v[2], v[3]);
@@ -616,8 +685,9 @@ attention_q8_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     } else if (!whole) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<uint4*>(slot + ((size_t)((c0 + e) >> 2) * QT_ITEM + irow) * 4) =
-                                make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+                            *reinterpret_cast<float4*>(slot + ((size_t)((c0 + e) >> 2) * QT_ITEM + irow) * 4) =
+                                make_float4(__uint_as_float(w[e]) * up_r, __uint_as_float(w[e + 1]) * up_r,
+                                            __uint_as_float(w[e + 2]) * up_r, __uint_as_float(w[e + 3]) * up_r);
                     }
                 }
                 if (!whole) {
@@ -727,6 +797,7 @@ static long long qt_layout(QtArgs* a, uint8_t* base, int n_tokens, int n_rows, i
     a->k16 = (__half*)take(vectors * hd * 2);
     a->v16 = (__half*)take(vectors * hd * 2);
     a->powers = (float2*)take(vectors / QT_KEYS * 8);
+    a->own = (float*)take(vectors * 8);
     return at;
 }
 // Bytes of scratch of a call over `n_rows` rows whose tokens see `stretch` positions (a multiple of 128).

@@ -438,6 +438,36 @@ def test_lengths_and_offsets_that_are_anything_on_tcgen05(window, dim, monkeypat
         assert rows((out.double().cpu() - want).abs() <= tol, [1, 3, 4, 5]).all() and torch.isfinite(out).all()
 
 
+@FORMATS
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("high", [10, 40, 80])
+@pytest.mark.parametrize("what", ["keys", "values", "both"])
+def test_a_later_token_far_above_the_others(what, high, dim, fmt, monkeypatch):
+    """Tokens in front of one whose key or value is 2^high times as large do not notice; the others see it."""
+    monkeypatch.setattr(K, "q8_on_tcgen05", lambda *a: True)
+    heads, kv = 4, 2
+    gen, rng = torch.Generator().manual_seed(1), np.random.RandomState(2)
+    ends, cu, at = [700], [0, 300], 560                       # position 560 is the token 160
+    table, n_pages = make_table(ends, 0, rng)
+    pages = make_pages(table, n_pages, ends, 0, kv, dim, fmt, gen)
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(torch.bfloat16).to(DEV)
+    page, place = table[0][at // PAGE], at % PAGE
+    if what != "values":
+        pages.k_scale[page, :, place] *= 2.0 ** high
+    if what != "keys":
+        pages.v_scale[page, :, place] *= 2.0 ** high
+    got = run_attention(q, pages, cu, ends, table, 0, heads, kv, dim, 0, 0.1)
+    want, *sizes = plain.attention(q, pages, cu, ends, table, 0, heads, kv, 0, 0.1)
+    # (where the far value is seen its weight is most of the result)
+    most = torch.zeros(cu[-1], 1, dtype=torch.float64)
+    ordinary = pages.v_scale.nan_to_num(0.0).clone()
+    ordinary[page, :, place] = 0
+    most[:160] = float(ordinary.max()) * plain.LIMIT[fmt]
+    most[160:] = float(pages.v_scale.nan_to_num(0.0).max()) * plain.LIMIT[fmt]
+    tol = plain.halves_tolerance(want, *sizes, most)
+    assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("heads", [6, 40])
 def test_portions_captured_twice_and_on_another_stream(heads, monkeypatch):
     monkeypatch.setattr(K, "q8_on_tcgen05", lambda *a: True)
