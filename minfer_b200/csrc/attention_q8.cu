@@ -479,14 +479,17 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
         }
         float x[KT][NT][4], w[KT][NT][4];
         float most = AQ_NEG, heaviest = 0.0f;
-        auto weigh = [&]() {
+        // AGAIN: with references of this step's scores.  A fused difference is off by what the reference was rounded by,
+        // which beyond 2^30 is more than a float's range of powers: then scores are rounded first, as references were
+        auto weigh = [&](auto again_tag) {
 #pragma unroll
             for (int k = 0; k < KT; ++k)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {          // 2 key + row
-                        x[k][n][e] = fmaf(sc[k][n][e], ks[k][e >> 1], neg[n][e & 1]);
+                        x[k][n][e] = decltype(again_tag)::value ? __fadd_rn(__fmul_rn(sc[k][n][e], ks[k][e >> 1]), neg[n][e & 1])
+                                                                : fmaf(sc[k][n][e], ks[k][e >> 1], neg[n][e & 1]);
                         // (a key or value that is not seen may have any scale: NaN must not get in)
                         if (EDGE && ((gone[k][n] >> e) & 1u)) x[k][n][e] = AQ_NEG;
                         w[k][n][e] = ex2(x[k][n][e]) * vs[k][e >> 1];
@@ -495,7 +498,7 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
                         heaviest = fmaxf(heaviest, w[k][n][e]);
                     }
         };
-        weigh();
+        weigh(std::false_type{});
         if (__any_sync(0xffffffffu, most > AQ_SCORE_ROOM || heaviest > AQ_WEIGHT_ROOM)) {
             // the references up to what is known now: the largest score first, then the largest weight
 #pragma unroll
@@ -507,7 +510,7 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
                     for (int k = 0; k < KT; ++k)
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
-                            if (!EDGE || !((gone[k][n] >> (2 * u + i)) & 1u)) top = fmaxf(top, sc[k][n][2 * u + i] * ks[k][u]);
+                            if (!EDGE || !((gone[k][n] >> (2 * u + i)) & 1u)) top = fmaxf(top, __fmul_rn(sc[k][n][2 * u + i], ks[k][u]));
                     const float before = -neg[n][i];
                     top = over_keys_max(top);
 #pragma unroll
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
                             if (!EDGE || !((gone[k][n] >> (2 * u + i)) & 1u))
-                                big = fmaxf(big, ex2(fmaf(sc[k][n][2 * u + i], ks[k][u], -top)) * vs[k][u]);
+                                big = fmaxf(big, ex2(__fadd_rn(__fmul_rn(sc[k][n][2 * u + i], ks[k][u]), -top)) * vs[k][u]);
                     big = fmaxf(over_keys_max(big), 8.1e-28f);         // (2^-90: values of zeros)
                     // (a row that has seen nothing yet keeps its infinity, one that is NaN its NaN)
                     const float m = fmaxf(before, top + __log2f(big));
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(AQ_WARPS * 32, MINB) attention_q8_mma_kernel(A
 #pragma unroll
                     for (int j = 0; j < OT; ++j) { o[n][j][i] *= f; o[n][j][2 + i] *= f; }
                 }
-            weigh();
+            weigh(std::true_type{});
         }
         uint32_t pb[KT][NT][2];
 #pragma unroll

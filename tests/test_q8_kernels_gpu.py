@@ -468,6 +468,24 @@ def test_a_later_token_far_above_the_others(what, high, dim, fmt, monkeypatch):
     assert ((got.double().cpu() - want).abs() <= tol).all()
 
 
+@FORMATS
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 96)])
+@pytest.mark.parametrize("high", [10, 40, 80])
+@pytest.mark.parametrize("longest", [300, 40000])
+def test_a_later_draft_with_a_key_far_above_the_others(longest, high, dtype, dim, fmt):
+    heads, kv = 4, 2
+    gen, rng = torch.Generator().manual_seed(1), np.random.RandomState(2)
+    ends, cu, at = [300, 100], [0, 6, 12], 297                # position 297 is the row's fourth token
+    table, n_pages = make_table(ends, 0, rng)
+    pages = make_pages(table, n_pages, ends, 0, kv, dim, fmt, gen)
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(dtype).to(DEV)
+    pages.k_scale[table[0][at // PAGE], :, at % PAGE] *= 2.0 ** high
+    got = run_attention(q, pages, cu, ends, table, 0, heads, kv, dim, 0, 0.1, max_end=longest)
+    want, *sizes = plain.attention(q, pages, cu, ends, table, 0, heads, kv, 0, 0.1)
+    tol = plain.attention_tolerance(want, *sizes, dtype, dim, fmt)
+    assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("heads", [6, 40])
 def test_portions_captured_twice_and_on_another_stream(heads, monkeypatch):
     monkeypatch.setattr(K, "q8_on_tcgen05", lambda *a: True)
