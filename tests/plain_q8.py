@@ -100,7 +100,7 @@ def attention_tolerance(want, mass, top, size, keys, dtype, dim, fmt):
 
 
 def halves_tolerance(want, mass, top, size, keys, most):
-    """The same where keys and values are rounded to halves with their scales (2^-11 each): a score is off by
+    """``attention_tolerance`` where keys and values are rounded to halves with their scales (2^-11 each): a score is off by
     2^-11 of the sum of its products' magnitudes and a probability relatively by twice that; probabilities are
     rounded to halves (2^-11), or by 2^-25 where the row's largest so far is 2^6 or more: 2^-31 of it, times a value
     of ``most`` at the largest, for each of n keys.  (A code of 2^-9 and a scale 2^-16 of the tile's largest are
@@ -109,15 +109,6 @@ def halves_tolerance(want, mass, top, size, keys, most):
     n = keys[:, None]
     rel = 2 * (2.0 ** -11 + 2.0 ** -14) * size + 2 * 2.0 ** -11 + 2.0 ** -14 + 2.0 ** -18 * (size + 1)
     return mass * rel[..., None] + (2.0 ** -31 * n * most)[..., None] + want.abs() * 2.0 ** -8 + 1e-37
-
-
-def read_back_tolerance(want, mass, top, size, keys):
-    """The same where keys and values are read back into bfloat16 first: each is rounded (2^-8, and its product
-    with the scale 2^-24 before), so a score is off by 2^-8 of the sum of its products' magnitudes and a
-    probability relatively by twice that (its own and the sum's); probabilities are rounded to bfloat16 for the
-    second product (2^-8), values are (2^-8), and so is the output (2^-8)."""
-    rel = 2 * (2.0 ** -8 + 2.0 ** -14) * size + 2 * 2.0 ** -8 + 2.0 ** -12
-    return mass * rel[..., None] + want.abs() * 2.0 ** -8 + 1e-37
 
 
 def softmax(row, temperature):
